@@ -233,6 +233,49 @@ constexpr int kChecksumParts = 4096;
 hipError_t launch_checksum(hipStream_t st, const void* src, size_t bytes, unsigned long long* part, int nparts,
                            unsigned long long* out, hipEvent_t read_done);
 
+// Causal attention over packed rows (attn_train.hip, attn_train_bwd.hip): sequence b's rows are qkv
+// rows b T .., q in columns 0 .. H hd, k in the Hk hd after them, v in the Hk hd after those; o and do
+// rows hold H hd columns.  The first `length` rows of a sequence count (all T unless ragged): the
+// others' outputs are zeros (lse -infinity), their inputs are not read.
+constexpr int kAttnTrainHead = 128, kAttnTrainLens = 64;
+struct AttnTrain {
+  const void* qkv;
+  void* out;         // forward's output, backward's input
+  float* lse;        // [B][H][T], as out
+  const void* dout;  // backward
+  void* dqkv;
+  float* dsum;  // [B][H][T] scratch: do . o of each row
+  int B, T, H, Hk, hd, qkv_cols, out_cols;
+  float scale;          // positive
+  int ragged;           // lengths in lens_dev, or in lens where that is null (B <= kAttnTrainLens)
+  const int* lens_dev;
+  int lens[kAttnTrainLens];
+};
+bool attn_train_fits(const AttnTrain& a);
+// whether every row of a head can be moved by 16 bytes (esize: bytes of an element)
+inline bool attn_train_vec(const AttnTrain& a, int esize) {
+  auto ok = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+  const int n = 16 / esize;
+  return a.hd % n == 0 && a.qkv_cols % n == 0 && a.out_cols % n == 0 && ok(a.qkv) && ok(a.out) && ok(a.dout) && ok(a.dqkv);
+}
+hipError_t launch_attn_forward(hipStream_t st, const AttnTrain& a, bool bf16, int cus);
+hipError_t launch_attn_backward(hipStream_t st, const AttnTrain& a, bool bf16, int cus);
+
+// Distillation from a teacher's top logits (distill.hip): row losses, and gradients where dlogits is
+// not null (it may be logits); then their sum in double into acc[0] (added) or acc[1].
+constexpr int kDistillTop = 1024;
+struct DistillArgs {
+  const void* logits;       // [T][V]
+  void* dlogits;            // [T][V] or null
+  const int* targets;       // [T], each below V or `ignore`
+  const int* top_ids;       // [T][K]; outside [0, V): an empty slot
+  const float* top_logits;  // [T][K]
+  float* row_loss;          // [T]
+  int T, V, K, ignore;
+  float tau, alpha, inv_count;
+};
+hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* acc, bool add);
+
 struct SampleArgs {
   const float* logits;  // [B][V] raw ForwardLast logits
   float* work;          // [B][V] scratch

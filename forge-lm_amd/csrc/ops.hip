@@ -76,6 +76,7 @@ __device__ __forceinline__ double block_sum_double(double s, double* red) {
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
 
 unsigned grid_for(size_t n) { return (unsigned)std::min<size_t>((n + kT - 1) / kT, 65536); }
 unsigned grid_vec(size_t n, bool v4) { return grid_for(v4 ? (n + 3) / 4 : n); }
@@ -1684,6 +1685,135 @@ int fh_op_adamw_step(fh_context* c, void* w, const void* g, void* m, void* v, in
     hipLaunchKernelGGL(k_adamw<1>, dim3(grid_for((size_t)n)), dim3(kT), 0, st_, fw, fg, fm, fv, (size_t)n, lr, beta1,
                        beta2, eps, weight_decay, bc1, bc2, decay);
   return op_launched("adamw step");
+}
+
+}  // extern "C"
+
+namespace {
+
+// The checks that attention's forward and backward share, and `a` filled from them.  lens stays
+// on the host here: attention_lens puts it where the kernels read it.
+int attention_args(const void* qkv, int qkv_cols, const void* out, int out_cols, const float* lse, const int32_t* lengths,
+                   int batch, int T, int n_heads, int n_kv_heads, int head_dim, float scale, int dtype, AttnTrain* a) {
+  OPS_ARG(qkv && out && lse, "null buffer");
+  OPS_ARG(dtype == FH_DTYPE_F32 || dtype == FH_DTYPE_BF16, "unknown dtype %d", dtype);
+  OPS_ARG(batch > 0 && T > 0 && n_heads > 0 && n_kv_heads > 0 && head_dim > 0,
+          "batch, T, n_heads, n_kv_heads and head_dim must be positive");
+  OPS_ARG(n_heads % n_kv_heads == 0, "n_heads (%d) must be a multiple of n_kv_heads (%d)", n_heads, n_kv_heads);
+  OPS_ARG(isfinite(scale) && scale > 0.f, "scale must be finite and positive");
+  OPS_ARG(qkv_cols >= ((int64_t)n_heads + 2 * (int64_t)n_kv_heads) * head_dim, "qkv rows of %d columns do not hold the heads",
+          qkv_cols);
+  OPS_ARG(out_cols >= (int64_t)n_heads * head_dim, "output rows of %d columns do not hold the heads", out_cols);
+  if (head_dim > kAttnTrainHead)
+    return set_err(FH_ERR_UNSUPPORTED, "head_dim above %d is not supported", kAttnTrainHead);
+  *a = AttnTrain{};
+  a->qkv = qkv, a->out = const_cast<void*>(out), a->lse = const_cast<float*>(lse);
+  a->B = batch, a->T = T, a->H = n_heads, a->Hk = n_kv_heads, a->hd = head_dim;
+  a->qkv_cols = qkv_cols, a->out_cols = out_cols, a->scale = scale;
+  if (!attn_train_fits(*a))
+    return set_err(FH_ERR_UNSUPPORTED, "batch * n_heads * T, or the rows' columns, are past this build's limits");
+  if (lengths) {
+    for (int b = 0; b < batch; b++)
+      if (lengths[b] < 0 || lengths[b] > T)
+        return set_err(FH_ERR_RANGE, "length %d of sequence %d outside [0,%d]", lengths[b], b, T);
+    a->ragged = 1;
+    if (batch <= kAttnTrainLens) std::memcpy(a->lens, lengths, (size_t)batch * sizeof(int32_t));
+  }
+  return FH_OK;
+}
+
+bool element_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == FH_DTYPE_BF16 ? 1 : 3)) == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int fh_op_attention_forward(fh_context* c, const void* qkv, int qkv_cols, void* out, int out_cols, float* lse,
+                            const int32_t* lengths, int batch, int T, int n_heads, int n_kv_heads, int head_dim, float scale,
+                            int dtype) {
+  OPS_ARG(c, "null context");
+  AttnTrain a;
+  FH_TRY(attention_args(qkv, qkv_cols, out, out_cols, lse, lengths, batch, T, n_heads, n_kv_heads, head_dim, scale, dtype, &a));
+  OPS_ARG(element_aligned(qkv, dtype) && element_aligned(out, dtype) && aligned4(lse), "buffer not aligned to its elements");
+  OPS_ARG(out != qkv && (const void*)lse != qkv && (void*)lse != out, "the outputs must be buffers of their own");
+  OPS_PROLOGUE(c);
+  if (lengths && batch > kAttnTrainLens) {
+    int* dev = nullptr;
+    FH_TRY(upload_ints(c, ops_, lengths, (size_t)batch, &dev));
+    a.lens_dev = dev;
+  }
+  HIP_TRY(launch_attn_forward(st_, a, dtype == FH_DTYPE_BF16, context_cus(c)));
+  return FH_OK;
+}
+
+int fh_op_attention_backward(fh_context* c, const void* dout, const void* qkv, int qkv_cols, const void* out, int out_cols,
+                             const float* lse, void* dqkv, const int32_t* lengths, int batch, int T, int n_heads,
+                             int n_kv_heads, int head_dim, float scale, int dtype) {
+  OPS_ARG(c, "null context");
+  AttnTrain a;
+  OPS_ARG(dout && dqkv, "null buffer");
+  FH_TRY(attention_args(qkv, qkv_cols, out, out_cols, lse, lengths, batch, T, n_heads, n_kv_heads, head_dim, scale, dtype, &a));
+  OPS_ARG(element_aligned(qkv, dtype) && element_aligned(out, dtype) && element_aligned(dout, dtype) &&
+              element_aligned(dqkv, dtype) && aligned4(lse),
+          "buffer not aligned to its elements");
+  OPS_ARG(dqkv != qkv && dqkv != out && dqkv != dout && dqkv != (const void*)lse, "dqkv must be a buffer of its own");
+  OPS_PROLOGUE(c);
+  a.dout = dout, a.dqkv = dqkv;
+  const size_t sums = (size_t)batch * n_heads * T;
+  const bool upload = lengths && batch > kAttnTrainLens;
+  void* p = nullptr;
+  FH_TRY(ops_scratch(c, ops_, (sums + (upload ? (size_t)batch : 0)) * 4, &p));
+  a.dsum = static_cast<float*>(p);
+  if (upload) {
+    int* dev = reinterpret_cast<int*>(a.dsum + sums);
+    FH_TRY(copy_ints(c, ops_, lengths, (size_t)batch, dev));
+    a.lens_dev = dev;
+  }
+  HIP_TRY(launch_attn_backward(st_, a, dtype == FH_DTYPE_BF16, context_cus(c)));
+  return FH_OK;
+}
+
+int fh_op_distill_loss(fh_context* c, const void* logits, const int32_t* targets, const int32_t* top_ids_dev,
+                       const float* top_logits_dev, void* dlogits, int T, int V, int K, int ignore_index, float temperature,
+                       float alpha, int dtype, float* loss) {
+  OPS_ARG(c, "null context");
+  OPS_ARG(logits && targets && top_ids_dev && top_logits_dev && loss, "null buffer");
+  OPS_ARG(dtype == FH_DTYPE_F32 || dtype == FH_DTYPE_BF16, "unknown dtype %d", dtype);
+  OPS_ARG(T > 0 && V > 0 && K > 0, "T, V and K must be positive");
+  OPS_ARG(isfinite(temperature) && temperature > 0.f, "temperature must be finite and positive");
+  OPS_ARG(alpha >= 0.f && alpha <= 1.f, "alpha must be between 0 and 1");
+  OPS_ARG(element_aligned(logits, dtype) && element_aligned(dlogits, dtype) && aligned4(top_ids_dev) && aligned4(top_logits_dev),
+          "buffer not aligned to its elements");
+  if (K > kDistillTop) return set_err(FH_ERR_UNSUPPORTED, "more than %d teacher logits per row are not supported", kDistillTop);
+  if (T >= 1 << 24) return set_err(FH_ERR_UNSUPPORTED, "2^24 rows and more are not supported");
+  int count = 0;
+  for (int t = 0; t < T; t++) {
+    if (targets[t] == ignore_index) continue;
+    if (targets[t] < 0 || targets[t] >= V)
+      return set_err(FH_ERR_RANGE, "target %d at position %d outside [0,%d)", targets[t], t, V);
+    count++;
+  }
+  OPS_PROLOGUE(c);
+  void* p = nullptr;
+  FH_TRY(ops_scratch(c, ops_, (size_t)T * (sizeof(int32_t) + sizeof(float)), &p));
+  int* dt = static_cast<int*>(p);
+  FH_TRY(copy_ints(c, ops_, targets, (size_t)T, dt));
+  DistillArgs a{};
+  a.logits = logits, a.dlogits = dlogits, a.targets = dt, a.top_ids = top_ids_dev, a.top_logits = top_logits_dev;
+  a.row_loss = reinterpret_cast<float*>(dt + T);
+  a.T = T, a.V = V, a.K = K, a.ignore = ignore_index, a.tau = temperature, a.alpha = alpha;
+  a.inv_count = count ? 1.f / (float)count : 0.f;
+  HIP_TRY(launch_distill(st_, a, dtype == FH_DTYPE_BF16, ops_->acc, ops_->accumulating));
+  *loss = 0.f;
+  if (ops_->accumulating) {  // the loss stays on the device until the accumulation ends
+    ops_->accumulated_targets += count;
+    return FH_OK;
+  }
+  double sum = 0;
+  HIP_TRY(hipMemcpyAsync(&sum, ops_->acc + 1, sizeof(double), hipMemcpyDeviceToHost, st_));
+  HIP_TRY(hipStreamSynchronize(st_));
+  if (count) *loss = (float)(sum / count);
+  return FH_OK;
 }
 
 }  // extern "C"

@@ -46,6 +46,8 @@ EXPORTS = (
     "fh_op_causal_mask", "fh_op_cross_entropy_forward", "fh_op_begin_loss_accumulation",
     "fh_op_end_loss_accumulation", "fh_op_cross_entropy_backward", "fh_op_sum_squares",
     "fh_op_global_sum_squares", "fh_op_adamw_step",
+    # beyond ITensorBackend
+    "fh_op_attention_forward", "fh_op_attention_backward", "fh_op_distill_loss",
 )
 
 
@@ -162,6 +164,9 @@ def lib():
     L.fh_op_sum_squares.argtypes = [vp, vp, i64, P(f64)]
     L.fh_op_global_sum_squares.argtypes = [vp, P(vp), P(i64), ci, P(f64)]
     L.fh_op_adamw_step.argtypes = [vp, vp, vp, vp, vp, i64, cf, cf, cf, cf, cf, ci, ci]
+    L.fh_op_attention_forward.argtypes = [vp, vp, ci, vp, ci, vp, vp, ci, ci, ci, ci, ci, cf, ci]
+    L.fh_op_attention_backward.argtypes = [vp, vp, vp, ci, vp, ci, vp, vp, vp, ci, ci, ci, ci, ci, cf, ci]
+    L.fh_op_distill_loss.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, cf, cf, ci, P(f32)]
     _lib = L
     return L
 

@@ -13,6 +13,7 @@ Names, argument meaning and error behaviour follow the reference:
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Callable, Optional, Sequence
 
@@ -158,6 +159,58 @@ class Random:
         self._pos += n
 
 
+def _dtype(name: str) -> int:
+    return {"f32": N.FH_DTYPE_F32, "fp32": N.FH_DTYPE_F32, "bf16": N.FH_DTYPE_BF16}[name]
+
+
+def _address(buf):
+    """A DeviceBuffer's device address, or the address itself."""
+    return buf.ptr if isinstance(buf, DeviceBuffer) else buf
+
+
+def _room(*needs) -> None:
+    """Checks the sizes of those of (name, buffer, bytes) that are DeviceBuffers."""
+    for name, buf, nbytes in needs:
+        if isinstance(buf, DeviceBuffer) and buf.nbytes < nbytes:
+            raise ValueError(f"{name} needs {nbytes} bytes, the buffer has {buf.nbytes}")
+
+
+@dataclass
+class _Attention:
+    qkv_cols: int
+    out_cols: int
+    kv: int
+    scale: float
+    dtype: int
+    host: Optional[np.ndarray]
+
+    @property
+    def lengths(self):
+        return None if self.host is None else self.host.ctypes.data
+
+
+def _attention(qkv, out, lse, batch, T, n_heads, head_dim, n_kv_heads, lengths, scale, qkv_cols, out_cols, dtype,
+               dout=None, dqkv=None) -> _Attention:
+    """The defaults and the buffers' sizes of an attention call."""
+    kv = n_heads if n_kv_heads is None else n_kv_heads
+    qkv_cols = (n_heads + 2 * kv) * head_dim if qkv_cols is None else qkv_cols
+    out_cols = n_heads * head_dim if out_cols is None else out_cols
+    scale = (1.0 / math.sqrt(head_dim) if head_dim > 0 else 1.0) if scale is None else scale
+    dt = _dtype(dtype)
+    host = None
+    if lengths is not None:
+        host = np.ascontiguousarray(lengths, np.int32).reshape(-1)
+        if host.size != batch:
+            raise ValueError(f"{batch} lengths are needed, got {host.size}")
+    rows, es = max(0, batch) * max(0, T), 2 if dt == N.FH_DTYPE_BF16 else 4
+    wide = max(0, rows - 1) * es
+    in_row, out_row = (n_heads + 2 * kv) * head_dim * es, n_heads * head_dim * es
+    _room(("qkv", qkv, wide * qkv_cols + in_row), ("dqkv", dqkv, wide * qkv_cols + in_row),
+          ("out", out, wide * out_cols + out_row), ("dout", dout, wide * out_cols + out_row),
+          ("lse", lse, rows * max(0, n_heads) * 4))
+    return _Attention(qkv_cols, out_cols, kv, float(scale), dt, host)
+
+
 class HipBackend:
     """One device + stream (the `hip` backend behind ITensorBackend's selection)."""
 
@@ -190,6 +243,47 @@ class HipBackend:
         if a.nbytes < M * K * 4 or b.nbytes < K * N_ * esz or y.nbytes < M * N_ * 4:
             raise ValueError("buffer smaller than the product's operands")
         N.check(N.lib().fh_matmul_nn(self._ctx, a.ptr, b.ptr, y.ptr, M, K, N_, dt, int(bool(accumulate))))
+
+    def attention_forward(self, qkv, out, lse, batch: int, T: int, n_heads: int, head_dim: int,
+                          n_kv_heads: Optional[int] = None, lengths: Optional[Sequence[int]] = None,
+                          scale: Optional[float] = None, qkv_cols: Optional[int] = None, out_cols: Optional[int] = None,
+                          dtype: str = "f32") -> None:
+        """Causal attention of packed q, k, v rows (fh_op_attention_forward): out rows and each row's log of
+        its softmax sum (lse, fp32).  Buffers are DeviceBuffers or device addresses; scale defaults to
+        1 / sqrt(head_dim), the widths to the packed ones, lengths to T each."""
+        a = _attention(qkv, out, lse, batch, T, n_heads, head_dim, n_kv_heads, lengths, scale, qkv_cols, out_cols, dtype)
+        N.check(N.lib().fh_op_attention_forward(self._ctx, _address(qkv), a.qkv_cols, _address(out), a.out_cols,
+                                                _address(lse), a.lengths, batch, T, n_heads, a.kv, head_dim, a.scale,
+                                                a.dtype))
+
+    def attention_backward(self, dout, qkv, out, lse, dqkv, batch: int, T: int, n_heads: int, head_dim: int,
+                           n_kv_heads: Optional[int] = None, lengths: Optional[Sequence[int]] = None,
+                           scale: Optional[float] = None, qkv_cols: Optional[int] = None,
+                           out_cols: Optional[int] = None, dtype: str = "f32") -> None:
+        """The gradient dqkv of attention_forward's inputs from dout and its outputs (fh_op_attention_backward)."""
+        a = _attention(qkv, out, lse, batch, T, n_heads, head_dim, n_kv_heads, lengths, scale, qkv_cols, out_cols, dtype,
+                       dout, dqkv)
+        N.check(N.lib().fh_op_attention_backward(self._ctx, _address(dout), _address(qkv), a.qkv_cols, _address(out),
+                                                 a.out_cols, _address(lse), _address(dqkv), a.lengths, batch, T, n_heads,
+                                                 a.kv, head_dim, a.scale, a.dtype))
+
+    def distill_loss(self, logits, targets: Sequence[int], top_ids, top_logits, dlogits, T: int, V: int, K: int,
+                     ignore_index: int = -1, temperature: float = 1.0, alpha: float = 1.0, dtype: str = "f32") -> float:
+        """Mean distillation loss against a teacher's top logits and hard targets, and its gradient where
+        dlogits is not None (fh_op_distill_loss).  Buffers are DeviceBuffers or device addresses: logits and
+        dlogits [T, V] of dtype, top_ids [T, K] int32, top_logits [T, K] fp32."""
+        dt = _dtype(dtype)
+        tg = np.ascontiguousarray(targets, np.int32).reshape(-1)
+        if tg.size < T:
+            raise ValueError(f"{T} targets are needed, got {tg.size}")
+        rows = max(0, T) * max(0, V) * (2 if dt == N.FH_DTYPE_BF16 else 4)
+        _room(("logits", logits, rows), ("dlogits", dlogits, rows), ("top_ids", top_ids, max(0, T) * max(0, K) * 4),
+              ("top_logits", top_logits, max(0, T) * max(0, K) * 4))
+        loss = ctypes.c_float()
+        N.check(N.lib().fh_op_distill_loss(self._ctx, _address(logits), tg.ctypes.data, _address(top_ids),
+                                           _address(top_logits), None if dlogits is None else _address(dlogits), T, V, K,
+                                           int(ignore_index), float(temperature), float(alpha), dt, ctypes.byref(loss)))
+        return float(loss.value)
 
     def dispose(self):
         if self._ctx:

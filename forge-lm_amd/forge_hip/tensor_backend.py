@@ -15,6 +15,7 @@ kernels on the stale device copy, as the contract states.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 from typing import Optional, Sequence
 
@@ -333,6 +334,74 @@ class HipTensorBackend:
         pp = self._read(probs)
         pd = self._write(dLogits, preserve=dLogits is probs)
         N.check(N.lib().fh_op_cross_entropy_backward(self._ctx, pp, tg.ctypes.data, pd, T, V, ignoreIndex))
+
+    # ---- attention and distillation without [T, T] or [T, V] intermediates (no reference counterpart) ----
+    @staticmethod
+    def _fits(name, t, rows, cols):
+        if t.Length < rows * cols:
+            raise ValueError(f"{name} of {t.Length} floats does not hold {rows} rows of {cols}")
+
+    def _attention_shape(self, qkv, output, lse, batch, T, nHeads, headDim, nKvHeads, lengths, scale):
+        kv = nHeads if nKvHeads is None else nKvHeads
+        for name, t, cols in (("qkv", qkv, (nHeads + 2 * kv) * headDim), ("output", output, nHeads * headDim)):
+            if t.Cols < cols:
+                raise ValueError(f"{name} rows of {t.Cols} columns do not hold the heads")
+            self._fits(name, t, batch * T, t.Cols)
+        self._fits("lse", lse, batch * nHeads, T)
+        ln = None if lengths is None else self._ints(lengths)
+        if ln is not None and ln.size != batch:
+            raise ValueError(f"{batch} lengths are needed, got {ln.size}")
+        scale = (1.0 / math.sqrt(headDim) if headDim > 0 else 1.0) if scale is None else float(scale)
+        return kv, ln, scale
+
+    def AttentionForward(self, qkv, output, lse, batch, T, nHeads, headDim, nKvHeads=None, lengths=None, scale=None):
+        """Causal attention of qkv rows as PackQkvHeads reads them (k and v of nKvHeads heads each): output
+        rows, and lse [batch, nHeads, T], the log of each row's softmax sum.  scale: 1 / sqrt(headDim)."""
+        kv, ln, scale = self._attention_shape(qkv, output, lse, batch, T, nHeads, headDim, nKvHeads, lengths, scale)
+        pq = self._read(qkv)
+        po = self._write(output, preserve=output.Length != batch * T * nHeads * headDim)
+        N.check(N.lib().fh_op_attention_forward(self._ctx, pq, qkv.Cols, po, output.Cols,
+                                                self._write(lse, preserve=lse.Length != batch * nHeads * T),
+                                                None if ln is None else ln.ctypes.data, batch, T, nHeads, kv, headDim,
+                                                scale, N.FH_DTYPE_F32))
+
+    def AttentionBackward(self, dOut, qkv, output, lse, dQkv, batch, T, nHeads, headDim, nKvHeads=None, lengths=None,
+                          scale=None):
+        """dQkv (qkv's layout, overwritten) from dOut and AttentionForward's inputs and outputs: the
+        probabilities are computed again from lse."""
+        kv, ln, scale = self._attention_shape(qkv, output, lse, batch, T, nHeads, headDim, nKvHeads, lengths, scale)
+        if dOut.Cols != output.Cols or dQkv.Cols != qkv.Cols:
+            raise ValueError("dOut and dQkv need the rows of output and qkv")
+        self._fits("dOut", dOut, batch * T, dOut.Cols)
+        self._fits("dQkv", dQkv, batch * T, dQkv.Cols)
+        pd, pq, po, pl = (self._read(t) for t in (dOut, qkv, output, lse))
+        pw = self._write(dQkv, preserve=dQkv.Length != batch * T * (nHeads + 2 * kv) * headDim)
+        N.check(N.lib().fh_op_attention_backward(self._ctx, pd, pq, qkv.Cols, po, output.Cols, pl, pw,
+                                                 None if ln is None else ln.ctypes.data, batch, T, nHeads, kv, headDim,
+                                                 scale, N.FH_DTYPE_F32))
+
+    def DistillLoss(self, logits, targets, topIds, topLogits, dLogits, T, V, K, ignoreIndex, temperature=1.0,
+                    alpha=1.0) -> float:
+        """The mean of alpha * temperature^2 * KL(teacher || student) + (1 - alpha) * cross-entropy over the
+        positions with a target, and its gradient in dLogits (None: the loss alone; may be logits).  topIds: a
+        DeviceBuffer of [T, K] int32 (outside [0, V): an empty slot), topLogits its [T, K] logits.  Inside a loss
+        accumulation the loss is returned by its end, as CrossEntropyForward's is."""
+        tg = self._ints(targets)
+        if tg.size < T:
+            raise ValueError(f"{T} targets are needed, got {tg.size}")
+        for name, t, cols in (("logits", logits, V), ("dLogits", dLogits, V), ("topLogits", topLogits, K)):
+            if t is not None:
+                self._fits(name, t, T, cols)
+        if topIds.nbytes < T * K * 4:
+            raise ValueError(f"topIds needs {T * K * 4} bytes, the buffer has {topIds.nbytes}")
+        pz, pt = self._read(logits), self._read(topLogits)
+        pd = None
+        if dLogits is not None:
+            pd = self._write(dLogits, preserve=dLogits is logits or dLogits.Length != T * V)
+        loss = ctypes.c_float()
+        N.check(N.lib().fh_op_distill_loss(self._ctx, pz, tg.ctypes.data, topIds.ptr, pt, pd, T, V, K, int(ignoreIndex),
+                                           float(temperature), float(alpha), N.FH_DTYPE_F32, ctypes.byref(loss)))
+        return float(loss.value)
 
     # ---- reductions, optimizer, housekeeping -----------------------------------------------------
     def Zero(self, t):

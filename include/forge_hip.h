@@ -329,6 +329,41 @@ int fh_op_global_sum_squares(fh_context* ctx, const void* const* xs, const int64
 int fh_op_adamw_step(fh_context* ctx, void* w, const void* g, void* m, void* v, int64_t n, float lr, float beta1,
                      float beta2, float eps, float weight_decay, int step, int is_matrix);
 
+/* ---- beyond ITensorBackend: a training step without [T, T] or [T, V] intermediates ----
+ * No counterpart in the reference, whose attention stores the probabilities of every head
+ * (MultiHeadAttention.Forward, src/LLM.Core/Layers/Layers.cs:191-229).  The conventions are those of
+ * the op entry points above; buffers are fp32 or bf16 (dtype), statistics and sums fp32.
+ *
+ * Causal attention of `batch` sequences of T rows.  A qkv row (qkv_cols wide) holds q of n_heads
+ * heads from column 0, then k and v of n_kv_heads heads each, head_dim (at most 128) columns to a
+ * head, as fh_op_pack_qkv_heads reads them; query heads h n_heads / n_kv_heads .. share k/v head h.
+ * out rows (out_cols wide) hold n_heads * head_dim columns.  lse [batch][n_heads][T] is the log of each
+ * row's sum of exp(scale * score), which the backward pass takes in place of the probabilities.
+ * lengths (host, or NULL: all T): the first lengths[b] rows of sequence b count; out rows past them are
+ * zeros and their lse -infinity, and their q, k, v are not read.  out and lse must not overlap qkv; the
+ * other columns of out rows are left as they are.  scale: finite and positive. */
+int fh_op_attention_forward(fh_context* ctx, const void* qkv, int qkv_cols, void* out, int out_cols, float* lse,
+                            const int32_t* lengths, int batch, int T, int n_heads, int n_kv_heads, int head_dim,
+                            float scale, int dtype);
+/* Its backward pass: dqkv (qkv's layout, overwritten; rows past a length are zeros, other columns left
+ * as they are) from dout (out's layout) and the forward's qkv, out and lse.  dqkv must not overlap an
+ * input.  Sums run in a fixed order: the same inputs give the same bits. */
+int fh_op_attention_backward(fh_context* ctx, const void* dout, const void* qkv, int qkv_cols, const void* out,
+                             int out_cols, const float* lse, void* dqkv, const int32_t* lengths, int batch, int T,
+                             int n_heads, int n_kv_heads, int head_dim, float scale, int dtype);
+/* Distillation from a teacher's top logits, next to CrossEntropyForward / Backward: the mean over the
+ * positions with a target (host array of T; ignore_index: none) of
+ *   alpha * temperature^2 * KL(teacher || student) + (1 - alpha) * cross-entropy(target)
+ * where the student is softmax(logits / temperature) over all V and the teacher softmax(top_logits /
+ * temperature) over the position's K slots (at most 1024).  top_ids [T][K] and top_logits [T][K] are
+ * device buffers; a slot whose id is outside [0, V) is empty, slots of one id add up, and a position whose
+ * slots are all empty (or all -infinity) has no KL term.  dlogits (device, logits' type; NULL: the loss
+ * alone; may be logits) receives the gradient, zeros at ignored positions.  *loss as
+ * fh_op_cross_entropy_forward gives it, the loss accumulation included. */
+int fh_op_distill_loss(fh_context* ctx, const void* logits, const int32_t* targets, const int32_t* top_ids_dev,
+                       const float* top_logits_dev, void* dlogits, int T, int V, int K, int ignore_index,
+                       float temperature, float alpha, int dtype, float* loss);
+
 #ifdef __cplusplus
 }
 #endif
