@@ -12,29 +12,24 @@ namespace fh {
 
 namespace {
 
-// KS == 1: four waves of 32 queries each share the key tiles.  KS == 4: the four waves own the same
-// 32 queries, take a quarter of each key tile, and their sums are joined at the end.
 template <typename E, int HD, int KS, bool VEC>
 __global__ __launch_bounds__(256) void k_attn_forward(const AttnTrain a) {
   typedef AtMma<E, HD> M;
-  constexpr int BQ = 128 / KS;
-  constexpr int SR = KS == 4 ? 128 : sizeof(E) == 4 && HD == 128 ? 32 : 64;  // keys of a tile
-  constexpr int NS = SR / (32 * KS);                                         // 32-key parts of a wave
-  constexpr int kTiles = 2 * SR * M::kStride * sizeof(E), kJoin = KS == 4 ? 4 * 32 * (HD + 3) * 4 : 0;
-  __shared__ __align__(16) char smem[kTiles > kJoin ? kTiles : kJoin];
-  E* Ks = reinterpret_cast<E*>(smem);
-  E* Vs = Ks + SR * M::kStride;
+  typedef AtPlan<E, HD, KS, VEC> P;
+  constexpr int kJoin = KS == 4 ? 4 * 32 * (HD + 3) * 4 : 0;
+  __shared__ __align__(1024) char smem[P::kBytes > kJoin ? P::kBytes : kJoin], odd[P::kBufs == 2 ? P::kBytes : 16];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nqb = (a.T + BQ - 1) / BQ;
+  const int nqb = (a.T + P::kOwn - 1) / P::kOwn;
   const AtBlock at = at_block(blockIdx.x, a.B * a.H);
   const int b = at.g / a.H, h = at.g % a.H, kvh = h / (a.H / a.Hk);
-  const int t0 = (nqb - 1 - at.blk) * BQ, len = at_len(a, b);
+  const int t0 = (nqb - 1 - at.blk) * P::kOwn, len = at_len(a, b);
   const int qw0 = t0 + (KS == 1 ? 32 * w : 0), q = qw0 + (lane & 31);
   const E* seq = static_cast<const E*>(a.qkv) + (size_t)b * a.T * a.qkv_cols;
   const E* kb = seq + (size_t)(a.H + kvh) * a.hd;
   const E* vb = kb + (size_t)a.Hk * a.hd;
   const float sl2 = a.scale * kLog2e;
+  const int mine = KS == 4 ? w * 2 * P::kTile : 0;  // this wave's K and V tiles in a buffer
 
   at_f32x16 o[HD / 32];
 #pragma unroll
@@ -44,25 +39,30 @@ __global__ __launch_bounds__(256) void k_attn_forward(const AttnTrain a) {
   if (t0 < len) {
     const typename M::Own own = M::template own<VEC>(
         at_rows(seq + (size_t)qw0 * a.qkv_cols + (size_t)h * a.hd, min(32, len - qw0), a.qkv_cols, a.hd), lane & 31, lane);
-    const int nkt = (min(t0 + BQ, len) - 1) / SR + 1;
-    for (int kt = 0; kt < nkt; kt++) {
-      const int k0 = kt * SR;
-      __syncthreads();
-      at_stage<E, HD, SR, VEC>(Ks, at_rows(kb + (size_t)k0 * a.qkv_cols, min(SR, len - k0), a.qkv_cols, a.hd), tid);
-      at_stage<E, HD, SR, VEC>(Vs, at_rows(vb + (size_t)k0 * a.qkv_cols, min(SR, len - k0), a.qkv_cols, a.hd), tid);
-      __syncthreads();
+    const int nkt = (min(t0 + P::kOwn, len) - 1) / P::kRows + 1;
+    auto fetch = [&](int kt, char* buf) {
+      const int k0 = kt * P::kRows + (KS == 4 ? 32 * w : 0), n = min(KS == 4 ? 32 : P::kRows, len - k0);
+      at_load<E, HD, KS, VEC>(reinterpret_cast<E*>(buf) + mine, at_rows(kb + (size_t)k0 * a.qkv_cols, n, a.qkv_cols, a.hd),
+                              at_rows(vb + (size_t)k0 * a.qkv_cols, n, a.qkv_cols, a.hd), w, lane);
+    };
+    auto compute = [&](int kt, const char* buf) {
+      const E *Ks = reinterpret_cast<const E*>(buf) + mine, *Vs = Ks + P::kTile;
 #pragma unroll
-      for (int n = 0; n < NS; n++) {
-        const int r0 = 32 * (KS == 1 ? n : w);  // the part's first row of the tile
-        if (k0 + r0 > qw0 + 31) continue;       // no query of this wave sees it
+      for (int n = 0; n < P::kParts; n++) {
+        const int k0 = kt * P::kRows + 32 * (KS == 1 ? n : w);  // the part's first key
+        if (k0 > qw0 + 31) continue;                            // no query of this wave sees it
         at_f32x16 s;
         at_zero(s);
-        M::rows(s, Ks, r0, own, lane);
+        M::rows(s, Ks, 32 * n, own, lane);
         float mt = -INFINITY;
-        const bool edge = k0 + r0 + 31 > qw0;
+        if (k0 + 31 > qw0) {  // the part crosses the diagonal
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (k0 + at_row(lane, r) > q) s[r] = -INFINITY;
+        }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          s[r] = !edge || k0 + r0 + at_row(lane, r) <= q ? s[r] * sl2 : -INFINITY;
+          s[r] *= sl2;
           mt = fmaxf(mt, s[r]);
         }
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
@@ -81,9 +81,10 @@ __global__ __launch_bounds__(256) void k_attn_forward(const AttnTrain a) {
         for (int dt = 0; dt < HD / 32; dt++)
 #pragma unroll
           for (int r = 0; r < 16; r++) o[dt][r] *= corr;
-        M::cols(o, Vs, r0, s, lane);
+        M::cols(o, Vs, 32 * n, s, lane);
       }
-    }
+    };
+    at_walk<P, KS>(nkt, smem, odd, fetch, compute);
     l += __shfl_xor(l, 32, 64);
   }
 

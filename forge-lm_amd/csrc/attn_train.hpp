@@ -137,8 +137,10 @@ template <int HD>
 struct AtMma<float, HD> {
   typedef float E;
   static constexpr int kChunks = HD / 4;
-  static constexpr int kStride = HD + 4;  // rows 4 banks apart
-  static __device__ __forceinline__ int at(int row, int chunk) { return row * kStride + 4 * chunk; }
+  static constexpr int kStride = HD;
+  // 16 rows of one chunk on distinct banks; the 32 lanes of a column read share a row
+  static __device__ __forceinline__ int swizzle(int row) { return HD == 32 ? (row >> 1) & 7 : row & 15; }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * kStride + 4 * (chunk ^ swizzle(row)); }
   struct Own {
     float v[HD / 2];  // own row l % 32, dims (l / 32) HD / 2 ..: a product step pairs dims d and d + HD / 2
   };
@@ -160,24 +162,30 @@ struct AtMma<float, HD> {
     return s;
   }
   static __device__ __forceinline__ void rows(at_f32x16& acc, const E* tile, int row0, const Own& o, int lane) {
-    const E* t = tile + (row0 + (lane & 31)) * kStride + (lane >> 5) * (HD / 2);
+    const int row = row0 + (lane & 31);
 #pragma unroll
     for (int c = 0; c < HD / 8; c++) {
-      const float4 a = *reinterpret_cast<const float4*>(t + 4 * c);
+      const float4 a = *reinterpret_cast<const float4*>(tile + at(row, (lane >> 5) * (HD / 8) + c));
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, o.v[4 * c], acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, o.v[4 * c + 1], acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, o.v[4 * c + 2], acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, o.v[4 * c + 3], acc, 0, 0, 0);
     }
   }
+  // row0 a multiple of 32: of a row's swizzle, bits 2 (HD 32) or 3 (`high`) and up are constants
   static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const E* tile, int row0, const at_f32x16& w,
                                               int lane) {
-    const E* t = tile + row0 * kStride + (lane & 31);
+    const int half = lane >> 5, c = (lane & 31) >> 2;
+    const E* t = tile + (row0 + 4 * half) * kStride + (lane & 3);
 #pragma unroll
-    for (int r = 0; r < 16; r++)
+    for (int r = 0; r < 16; r++) {
+      const int row = (r >> 2) * 8 + (r & 3), high = (r >> 2) & 1;
+      const int low = HD == 32 ? (c ^ (2 * half + ((r & 3) >> 1))) ^ (4 * high) : c ^ (4 * half + (r & 3));
 #pragma unroll
       for (int dt = 0; dt < HD / 32; dt++)
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(t[at_row(lane, r) * kStride + dt * 32], w[r], acc[dt], 0, 0, 0);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(t[row * kStride + 4 * low + (HD == 32 ? 0 : 32 * (dt ^ high))], w[r],
+                                                       acc[dt], 0, 0, 0);
+    }
   }
 };
 
@@ -185,13 +193,40 @@ struct AtMma<float, HD> {
 template <typename E, int HD, int SR, bool VEC>
 __device__ __forceinline__ void at_stage(E* tile, const AtRows<E>& m, int tid) {
   typedef AtMma<E, HD> M;
-  constexpr int N = SR * M::kChunks / 256;
-  at_u32x4 v[N];
 #pragma unroll
-  for (int i = 0; i < N; i++) v[i] = at_chunk<E, VEC>(m, (tid + 256 * i) / M::kChunks, (tid + 256 * i) % M::kChunks);
+  for (int i = 0; i < SR * M::kChunks / 256; i++) {
+    const int row = (tid + 256 * i) / M::kChunks, c = (tid + 256 * i) % M::kChunks;
+    *reinterpret_cast<at_u32x4*>(tile + M::at(row, c)) = at_chunk<E, VEC>(m, row, c);
+  }
+}
+
+// ROWS rows of m straight into an LDS tile: 1 KB pieces (64 lanes x 16 bytes, contiguous in LDS),
+// every WAVES-th of them from `first` by this wave.  A lane asks for the chunk whose place is its own.
+// Chunks past either end of m arrive as zeros.
+template <typename E, int HD, int ROWS, int WAVES>
+__device__ __forceinline__ void at_fetch(E* tile, const AtRows<E>& m, int first, int lane) {
+  typedef AtMma<E, HD> M;
+  constexpr int CE = 16 / sizeof(E), RP = 64 / M::kChunks, N = ROWS / RP / WAVES;
+  static_assert(N * RP * WAVES == ROWS, "pieces");
 #pragma unroll
-  for (int i = 0; i < N; i++)
-    *reinterpret_cast<at_u32x4*>(tile + M::at((tid + 256 * i) / M::kChunks, (tid + 256 * i) % M::kChunks)) = v[i];
+  for (int i = 0; i < N; i++) {
+    const int row0 = (first + WAVES * i) * RP, row = row0 + lane / M::kChunks;
+    const int c = (lane % M::kChunks) ^ M::swizzle(row);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(m.rsrc, (__attribute__((address_space(3))) void*)(tile + row0 * M::kStride), 16,
+                                             c * CE < m.hd ? row * m.stride + c * 16 : 0x7ffffff0, 0, 0, 0);
+  }
+}
+
+// This wave's requests have landed and its LDS reads are done; BLOCK: every wave's of the block.  (The
+// builtin, unlike a wait in inline assembly, also tells the compiler that nothing is in flight.)
+template <bool BLOCK>
+__device__ __forceinline__ void at_landed() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  if constexpr (BLOCK) __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // acc^T (dims x own rows) times f to row `row` (a pointer to its hd elements) of the lane's own row
@@ -215,6 +250,61 @@ __device__ __forceinline__ void at_store(E* row, const at_f32x16 (&acc)[HD / 32]
     }
 }
 
+// How a block goes through the axis it walks.  KS == 1: its four waves own 32 rows each of the other
+// axis and share tiles of kRows rows.  KS == 4: they own the same 32 rows and each walks every fourth
+// 32-row part through tiles of its own, without a barrier; their sums are joined at the end.
+// Tiles are requested one ahead into the other of two buffers (one buffer where two do not fit).
+template <typename E, int HD, int KS, bool VEC>
+struct AtPlan {
+  static constexpr int kOwn = 128 / KS;  // rows of a block
+  static constexpr int kRows = KS == 4 ? 128 : sizeof(E) == 4 && HD == 128 ? 32 : 64;
+  static constexpr int kParts = kRows / (32 * KS);     // 32-row parts of a wave
+  static constexpr int kTile = (KS == 4 ? 32 : kRows) * HD;  // elements of one operand's tile
+  static constexpr int kBufs = VEC && !(KS == 4 && sizeof(E) == 4 && HD == 128) ? 2 : 1;
+  static constexpr int kBytes = 2 * kTile * KS * (int)sizeof(E);  // a buffer: both operands, all waves
+};
+
+// The tiles of two operands into `tiles` (the second kTile elements on): by all four waves of the
+// block (KS == 1), or by this wave alone.
+template <typename E, int HD, int KS, bool VEC>
+__device__ __forceinline__ void at_load(E* tiles, const AtRows<E>& x, const AtRows<E>& y, int w, int lane) {
+  typedef AtPlan<E, HD, KS, VEC> P;
+  if constexpr (VEC) {
+    constexpr int ROWS = KS == 4 ? 32 : P::kRows, WAVES = KS == 4 ? 1 : 4;
+    at_fetch<E, HD, ROWS, WAVES>(tiles, x, KS == 4 ? 0 : w, lane);
+    at_fetch<E, HD, ROWS, WAVES>(tiles + P::kTile, y, KS == 4 ? 0 : w, lane);
+  } else {
+    static_assert(KS == 1, "element loads are shared by the block");
+    at_stage<E, HD, P::kRows, false>(tiles, x, 64 * w + lane);
+    at_stage<E, HD, P::kRows, false>(tiles + P::kTile, y, 64 * w + lane);
+  }
+}
+// The steps 0 .. n - 1 of a walk: step kt computes on a buffer whose tiles have landed while those of
+// kt + 1 are on their way to the other.  The two buffers are LDS variables of their own and appear by
+// name in code of their own, so that the compiler does not make the reads of one wait for the other.
+template <typename P, int KS, typename F, typename C>
+__device__ __forceinline__ void at_walk(int n, char* even, char* odd, const F& fetch, const C& compute) {
+  if constexpr (P::kBufs == 2) {
+    fetch(0, even);
+    for (int kt = 0; kt < n; kt += 2) {
+      at_landed<KS == 1>();
+      if (kt + 1 < n) fetch(kt + 1, odd);
+      compute(kt, even);
+      if (kt + 1 == n) break;
+      at_landed<KS == 1>();
+      if (kt + 2 < n) fetch(kt + 2, even);
+      compute(kt + 1, odd);
+    }
+  } else {
+    for (int kt = 0; kt < n; kt++) {
+      at_landed<KS == 1>();  // the last tile's reads are done
+      fetch(kt, even);
+      at_landed<KS == 1>();
+      compute(kt, even);
+    }
+  }
+}
+
 // Block -> (block of the axis, group = sequence * heads + head) of a causal launch over nblk * G
 // blocks; block 0 of the axis is the one with the most work, and is started first.  Workgroups reach
 // the 8 XCDs round-robin: when 8 divides G, an XCD takes whole neighbouring groups, so that what their
@@ -232,7 +322,7 @@ __device__ __forceinline__ AtBlock at_block(int L, int G) {
 
 __device__ __forceinline__ int at_len(const AttnTrain& a, int b) {
   if (!a.ragged) return a.T;
-  return a.lens_dev ? a.lens_dev[b] : a.lens[b];
+  return __builtin_amdgcn_readfirstlane(a.lens_dev ? a.lens_dev[b] : a.lens[b]);
 }
 
 }  // namespace fh

@@ -37,34 +37,43 @@ __device__ __forceinline__ void join_store(float* os, const at_f32x16 (&acc)[HD 
   }
 }
 
+// lse and D of the rows as the other kernel reads them, [head][32-row part][32 of lse * log2(e), 32 of
+// D]; rows past the length have lse +infinity (their p is 0) and D 0, parts past it are not written.
+__device__ __forceinline__ float* stat_part(const AttnTrain& a, size_t head, int row) {
+  return a.stats + (head * ((a.T + 31) / 32) + row / 32) * 64;
+}
+
 template <typename E, int HD, int KS, bool VEC>
 __global__ __launch_bounds__(256) void k_attn_backward_q(const AttnTrain a) {
   typedef AtMma<E, HD> M;
-  constexpr int BQ = 128 / KS;
-  constexpr int SR = KS == 4 ? 128 : sizeof(E) == 4 && HD == 128 ? 32 : 64;
-  constexpr int NS = SR / (32 * KS);
-  constexpr int kTiles = 2 * SR * M::kStride * sizeof(E), kJoin = KS == 4 ? 4 * 32 * (HD + 1) * 4 : 0;
-  __shared__ __align__(16) char smem[kTiles > kJoin ? kTiles : kJoin];
-  E* Ks = reinterpret_cast<E*>(smem);
-  E* Vs = Ks + SR * M::kStride;
+  typedef AtPlan<E, HD, KS, VEC> P;
+  constexpr int kJoin = KS == 4 ? 4 * 32 * (HD + 1) * 4 : 0;
+  __shared__ __align__(1024) char smem[P::kBytes > kJoin ? P::kBytes : kJoin], odd[P::kBufs == 2 ? P::kBytes : 16];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nqb = (a.T + BQ - 1) / BQ;
+  const int nqb = (a.T + P::kOwn - 1) / P::kOwn;
   const AtBlock at = at_block(blockIdx.x, a.B * a.H);
   const int b = at.g / a.H, h = at.g % a.H, kvh = h / (a.H / a.Hk);
-  const int t0 = (nqb - 1 - at.blk) * BQ, len = at_len(a, b);
+  const int t0 = (nqb - 1 - at.blk) * P::kOwn, len = at_len(a, b);
   const int qw0 = t0 + (KS == 1 ? 32 * w : 0), q = qw0 + (lane & 31);
   const size_t row0 = (size_t)b * a.T;
   const E* seq = static_cast<const E*>(a.qkv) + row0 * a.qkv_cols;
   const E* kb = seq + (size_t)(a.H + kvh) * a.hd;
   const E* vb = kb + (size_t)a.Hk * a.hd;
   const float sl2 = a.scale * kLog2e;
+  const int mine = KS == 4 ? w * 2 * P::kTile : 0;  // this wave's K and V tiles in a buffer
 
   at_f32x16 dq[HD / 32];
 #pragma unroll
   for (int dt = 0; dt < HD / 32; dt++) at_zero(dq[dt]);
 
   if (t0 < len) {
+    const int nkt = (min(t0 + P::kOwn, len) - 1) / P::kRows + 1;
+    auto fetch = [&](int kt, char* buf) {
+      const int k0 = kt * P::kRows + (KS == 4 ? 32 * w : 0), n = min(KS == 4 ? 32 : P::kRows, len - k0);
+      at_load<E, HD, KS, VEC>(reinterpret_cast<E*>(buf) + mine, at_rows(kb + (size_t)k0 * a.qkv_cols, n, a.qkv_cols, a.hd),
+                              at_rows(vb + (size_t)k0 * a.qkv_cols, n, a.qkv_cols, a.hd), w, lane);
+    };
     const int n = min(32, len - qw0);
     const typename M::Own own = M::template own<VEC>(
         at_rows(seq + (size_t)qw0 * a.qkv_cols + (size_t)h * a.hd, n, a.qkv_cols, a.hd), lane & 31, lane);
@@ -74,33 +83,30 @@ __global__ __launch_bounds__(256) void k_attn_backward_q(const AttnTrain a) {
     float D = M::dot(dout, M::template own<VEC>(at_rows(static_cast<const E*>(a.out) + orow, n, a.out_cols, a.hd),
                                                 lane & 31, lane));
     D += __shfl_xor(D, 32, 64);
-    if ((KS == 1 || w == 0) && lane < 32 && q < len) a.dsum[(size_t)at.g * a.T + q] = D;
-    const float lse2 = q < len ? a.lse[(size_t)at.g * a.T + q] * kLog2e : INFINITY;  // p = 0 past the length
-    const int nkt = (min(t0 + BQ, len) - 1) / SR + 1;
-    for (int kt = 0; kt < nkt; kt++) {
-      const int k0 = kt * SR;
-      __syncthreads();
-      at_stage<E, HD, SR, VEC>(Ks, at_rows(kb + (size_t)k0 * a.qkv_cols, min(SR, len - k0), a.qkv_cols, a.hd), tid);
-      at_stage<E, HD, SR, VEC>(Vs, at_rows(vb + (size_t)k0 * a.qkv_cols, min(SR, len - k0), a.qkv_cols, a.hd), tid);
-      __syncthreads();
+    const float lse2 = q < len ? a.lse[(size_t)at.g * a.T + q] * kLog2e : INFINITY;
+    if ((KS == 1 || w == 0) && qw0 < len) stat_part(a, at.g, qw0)[lane] = lane < 32 ? lse2 : D;
+    auto compute = [&](int kt, const char* buf) {
+      const E *Ks = reinterpret_cast<const E*>(buf) + mine, *Vs = Ks + P::kTile;
 #pragma unroll
-      for (int i = 0; i < NS; i++) {
-        const int r0 = 32 * (KS == 1 ? i : w);
-        if (k0 + r0 > qw0 + 31) continue;
+      for (int i = 0; i < P::kParts; i++) {
+        const int k0 = kt * P::kRows + 32 * (KS == 1 ? i : w);
+        if (k0 > qw0 + 31) continue;
         at_f32x16 s, dp;
         at_zero(s);
         at_zero(dp);
-        M::rows(s, Ks, r0, own, lane);
-        M::rows(dp, Vs, r0, dout, lane);
-        const bool edge = k0 + r0 + 31 > qw0;
+        M::rows(s, Ks, 32 * i, own, lane);
+        M::rows(dp, Vs, 32 * i, dout, lane);
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[r], sl2, -lse2));
-          s[r] = !edge || k0 + r0 + at_row(lane, r) <= q ? p * (dp[r] - D) : 0.f;
+        for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl2, -lse2)) * (dp[r] - D);
+        if (k0 + 31 > qw0) {  // the part crosses the diagonal
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (k0 + at_row(lane, r) > q) s[r] = 0.f;
         }
-        M::cols(dq, Ks, r0, s, lane);
+        M::cols(dq, Ks, 32 * i, s, lane);
       }
-    }
+    };
+    at_walk<P, KS>(nkt, smem, odd, fetch, compute);
   }
   E* dst = static_cast<E*>(a.dqkv) + row0 * a.qkv_cols + (size_t)h * a.hd;
   if constexpr (KS == 1) {
@@ -117,23 +123,20 @@ __global__ __launch_bounds__(256) void k_attn_backward_q(const AttnTrain a) {
 template <typename E, int HD, int KS, bool VEC>
 __global__ __launch_bounds__(256) void k_attn_backward_kv(const AttnTrain a) {
   typedef AtMma<E, HD> M;
-  constexpr int BK = 128 / KS;
-  constexpr int SR = KS == 4 ? 128 : sizeof(E) == 4 && HD == 128 ? 32 : 64;  // queries of a tile
-  constexpr int NS = SR / (32 * KS);
-  constexpr int kTiles = 2 * SR * M::kStride * sizeof(E), kJoin = KS == 4 ? 4 * 32 * (HD + 1) * 4 : 0;
-  __shared__ __align__(16) char smem[kTiles > kJoin ? kTiles : kJoin];
-  __shared__ __align__(16) float Ls[SR], Ds[SR];
-  E* Qs = reinterpret_cast<E*>(smem);
-  E* Os = Qs + SR * M::kStride;
+  typedef AtPlan<E, HD, KS, VEC> P;
+  constexpr int kJoin = KS == 4 ? 4 * 32 * (HD + 1) * 4 : 0;
+  __shared__ __align__(1024) char smem[P::kBytes > kJoin ? P::kBytes : kJoin], odd[P::kBufs == 2 ? P::kBytes : 16];
+  __shared__ __align__(1024) float stat[P::kRows / 32][64], stat_odd[P::kRows / 32][64];  // of a buffer's parts
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const AtBlock at = at_block(blockIdx.x, a.B * a.Hk);
   const int b = at.g / a.Hk, kvh = at.g % a.Hk, group = a.H / a.Hk;
-  const int k0 = at.blk * BK, len = at_len(a, b);
+  const int k0 = at.blk * P::kOwn, len = at_len(a, b);
   const int kw0 = k0 + (KS == 1 ? 32 * w : 0), key = kw0 + (lane & 31);
   const size_t row0 = (size_t)b * a.T;
   const E* seq = static_cast<const E*>(a.qkv) + row0 * a.qkv_cols;
   const float sl2 = a.scale * kLog2e;
+  const int mine = KS == 4 ? w * 2 * P::kTile : 0;  // this wave's Q and dO tiles in a buffer
 
   at_f32x16 dk[HD / 32], dv[HD / 32];
 #pragma unroll
@@ -142,54 +145,73 @@ __global__ __launch_bounds__(256) void k_attn_backward_kv(const AttnTrain a) {
     at_zero(dv[dt]);
   }
   if (k0 < len) {
+    const int nqt = (len - k0 + P::kRows - 1) / P::kRows, nt = nqt * group;  // a head's tiles, all tiles
+    int fg = 0, fq = k0;  // head of the group and first row of the tile to be fetched next
+    auto fetch = [&](int, char* buf) {
+      float(*sp)[64] = buf == smem ? stat : stat_odd;
+      const int h = kvh * group + fg, q0 = fq + (KS == 4 ? 32 * w : 0), n = min(KS == 4 ? 32 : P::kRows, len - q0);
+      const E* qb = seq + (size_t)q0 * a.qkv_cols + (size_t)h * a.hd;
+      const E* ob = static_cast<const E*>(a.dout) + (row0 + q0) * a.out_cols + (size_t)h * a.hd;
+      at_load<E, HD, KS, VEC>(reinterpret_cast<E*>(buf) + mine, at_rows(qb, n, a.qkv_cols, a.hd),
+                              at_rows(ob, n, a.out_cols, a.hd), w, lane);
+      // 32-row parts of the statistics: a wave's own, or one for each of the first waves
+      const int part = fq + 32 * w;
+      if ((KS == 4 || w < P::kRows / 32) && part < len) {
+        if constexpr (VEC)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              at_rows(stat_part(a, (size_t)b * a.H + h, part), 1, 64, 64).rsrc,
+              (__attribute__((address_space(3))) void*)&sp[w][0], 4, lane * 4, 0, 0, 0);
+        else
+          sp[w][lane] = stat_part(a, (size_t)b * a.H + h, part)[lane];
+      }
+      fq += P::kRows;
+      if (fq >= len) {
+        fq = k0;
+        fg++;
+      }
+    };
     const int n = min(32, len - kw0);
     const E* kb = seq + (size_t)kw0 * a.qkv_cols + (size_t)(a.H + kvh) * a.hd;
     const typename M::Own ko = M::template own<VEC>(at_rows(kb, n, a.qkv_cols, a.hd), lane & 31, lane);
     const typename M::Own vo =
         M::template own<VEC>(at_rows(kb + (size_t)a.Hk * a.hd, n, a.qkv_cols, a.hd), lane & 31, lane);
-    for (int g = 0; g < group; g++) {
-      const int h = kvh * group + g;
-      const E* qb = seq + (size_t)h * a.hd;
-      const E* ob = static_cast<const E*>(a.dout) + row0 * a.out_cols + (size_t)h * a.hd;
-      const float* lse = a.lse + ((size_t)b * a.H + h) * a.T;
-      const float* dsum = a.dsum + ((size_t)b * a.H + h) * a.T;
-      for (int q0 = k0; q0 < len; q0 += SR) {
-        __syncthreads();
-        at_stage<E, HD, SR, VEC>(Qs, at_rows(qb + (size_t)q0 * a.qkv_cols, min(SR, len - q0), a.qkv_cols, a.hd), tid);
-        at_stage<E, HD, SR, VEC>(Os, at_rows(ob + (size_t)q0 * a.out_cols, min(SR, len - q0), a.out_cols, a.hd), tid);
-        if (tid < SR) {
-          Ls[tid] = q0 + tid < len ? lse[q0 + tid] * kLog2e : INFINITY;  // p = 0 past the length
-          Ds[tid] = q0 + tid < len ? dsum[q0 + tid] : 0.f;
-        }
-        __syncthreads();
+    int q0 = k0;
+    auto compute = [&](int, const char* buf) {
+      const float(*sp)[64] = buf == smem ? stat : stat_odd;
+      const E *Qs = reinterpret_cast<const E*>(buf) + mine, *Os = Qs + P::kTile;
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-          const int r0 = 32 * (KS == 1 ? i : w);
-          if (q0 + r0 + 31 < kw0 || q0 + r0 >= len) continue;  // every query of it is before these keys, or past the length
-          at_f32x16 s, dp;
-          at_zero(s);
-          at_zero(dp);
-          M::rows(s, Qs, r0, ko, lane);
-          M::rows(dp, Os, r0, vo, lane);
-          const bool edge = q0 + r0 < kw0 + 31;
+      for (int i = 0; i < P::kParts; i++) {
+        const int part = KS == 1 ? i : w, r0 = q0 + 32 * part;  // the part's first query
+        if (r0 + 31 < kw0 || r0 >= len) continue;  // every query of it is before these keys, or past the length
+        at_f32x16 s, dp;
+        at_zero(s);
+        at_zero(dp);
+        M::rows(s, Qs, 32 * i, ko, lane);
+        M::rows(dp, Os, 32 * i, vo, lane);
+        const float* st = &sp[part][4 * (lane >> 5)];
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const int i0 = r0 + 8 * c + 4 * (lane >> 5);
-            const float4 ls = *reinterpret_cast<const float4*>(&Ls[i0]), ds = *reinterpret_cast<const float4*>(&Ds[i0]);
-            const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {ds.x, ds.y, ds.z, ds.w};
+        for (int c = 0; c < 4; c++) {
+          const float4 ls = *reinterpret_cast<const float4*>(st + 8 * c), ds = *reinterpret_cast<const float4*>(st + 32 + 8 * c);
+          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {ds.x, ds.y, ds.z, ds.w};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * c + e], sl2, -l4[e]));
-              const bool seen = !edge || key <= q0 + i0 + e;
-              s[4 * c + e] = seen ? p : 0.f;
-              dp[4 * c + e] = seen ? p * (dp[4 * c + e] - d4[e]) : 0.f;
-            }
+          for (int e = 0; e < 4; e++) {
+            const int r = 4 * c + e;
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl2, -l4[e]));
+            dp[r] = s[r] * (dp[r] - d4[e]);
           }
-          M::cols(dv, Os, r0, s, lane);
-          M::cols(dk, Qs, r0, dp, lane);
         }
+        if (r0 < kw0 + 31) {  // the part crosses the diagonal
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (key > r0 + at_row(lane, r)) s[r] = dp[r] = 0.f;
+        }
+        M::cols(dv, Os, 32 * i, s, lane);
+        M::cols(dk, Qs, 32 * i, dp, lane);
       }
-    }
+      q0 += P::kRows;
+      if (q0 >= len) q0 = k0;
+    };
+    at_walk<P, KS>(nt, smem, odd, fetch, compute);
   }
   E* dst = static_cast<E*>(a.dqkv) + row0 * a.qkv_cols + (size_t)(a.H + kvh) * a.hd;
   E* dstv = dst + (size_t)a.Hk * a.hd;
@@ -242,7 +264,7 @@ void backward(hipStream_t st, const AttnTrain& a, bool vec, int cus) {
 }  // namespace
 
 hipError_t launch_attn_backward(hipStream_t st, const AttnTrain& a, bool bf16, int cus) {
-  if (!attn_train_fits(a) || !a.qkv || !a.out || !a.lse || !a.dout || !a.dqkv || !a.dsum) return hipErrorInvalidValue;
+  if (!attn_train_fits(a) || !a.qkv || !a.out || !a.lse || !a.dout || !a.dqkv || !a.stats) return hipErrorInvalidValue;
   const bool vec = attn_train_vec(a, bf16 ? 2 : 4);
   if (bf16)
     backward<__bf16>(st, a, vec, cus);

@@ -244,7 +244,7 @@ struct AttnTrain {
   float* lse;        // [B][H][T], as out
   const void* dout;  // backward
   void* dqkv;
-  float* dsum;  // [B][H][T] scratch: do . o of each row
+  float* stats;  // backward's scratch, attn_train_stats(a) floats
   int B, T, H, Hk, hd, qkv_cols, out_cols;
   float scale;          // positive
   int ragged;           // lengths in lens_dev, or in lens where that is null (B <= kAttnTrainLens)
@@ -252,6 +252,7 @@ struct AttnTrain {
   int lens[kAttnTrainLens];
 };
 bool attn_train_fits(const AttnTrain& a);
+inline size_t attn_train_stats(const AttnTrain& a) { return (size_t)a.B * a.H * ((a.T + 31) / 32) * 64; }
 // whether every row of a head can be moved by 16 bytes (esize: bytes of an element)
 inline bool attn_train_vec(const AttnTrain& a, int esize) {
   auto ok = [](const void* p) { return ((uintptr_t)p & 15) == 0; };

@@ -1759,13 +1759,13 @@ int fh_op_attention_backward(fh_context* c, const void* dout, const void* qkv, i
   OPS_ARG(dqkv != qkv && dqkv != out && dqkv != dout && dqkv != (const void*)lse, "dqkv must be a buffer of its own");
   OPS_PROLOGUE(c);
   a.dout = dout, a.dqkv = dqkv;
-  const size_t sums = (size_t)batch * n_heads * T;
+  const size_t sums = attn_train_stats(a);
   const bool upload = lengths && batch > kAttnTrainLens;
   void* p = nullptr;
   FH_TRY(ops_scratch(c, ops_, (sums + (upload ? (size_t)batch : 0)) * 4, &p));
-  a.dsum = static_cast<float*>(p);
+  a.stats = static_cast<float*>(p);
   if (upload) {
-    int* dev = reinterpret_cast<int*>(a.dsum + sums);
+    int* dev = reinterpret_cast<int*>(a.stats + sums);
     FH_TRY(copy_ints(c, ops_, lengths, (size_t)batch, dev));
     a.lens_dev = dev;
   }
