@@ -13,6 +13,8 @@
 
 #include "kernels.hpp"
 
+#include <type_traits>
+
 namespace fh {
 
 typedef __bf16 at_bf16x8 __attribute__((ext_vector_type(8)));
@@ -20,9 +22,13 @@ typedef float at_f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int at_u32x4 __attribute__((ext_vector_type(4)));
 typedef short at_s16x4 __attribute__((ext_vector_type(4)));
 
+template <int I>
+constexpr std::integral_constant<int, I> at_int{};
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ int at_row(int lane, int r) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
+constexpr __device__ __forceinline__ int at_row0(int r) { return (r >> 2) * 8 + (r & 3); }  // of the lower lanes
+__device__ __forceinline__ int at_row(int lane, int r) { return at_row0(r) + (lane >> 5) * 4; }
 
 __device__ __forceinline__ void at_zero(at_f32x16& v) {
 #pragma unroll
@@ -98,37 +104,54 @@ struct AtMma<__bf16, HD> {
       for (int e = 0; e < 8; e++) s = fmaf((float)a.v[kk][e], (float)b.v[kk][e], s);
     return s;
   }
-  static __device__ __forceinline__ void rows(at_f32x16& acc, const E* tile, int row0, const Own& o, int lane) {
-    const int row = row0 + (lane & 31);
+  // 32 rows of a tile as the operand of `rows`
+  struct Rows {
+    at_bf16x8 v[HD / 16];
+  };
+  static __device__ __forceinline__ Rows load_rows(const E* tile, int row0, int lane) {
+    Rows f;
 #pragma unroll
     for (int kk = 0; kk < HD / 16; kk++)
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-          *reinterpret_cast<const at_bf16x8*>(tile + at(row, 2 * kk + (lane >> 5))), o.v[kk], acc, 0, 0, 0);
+      f.v[kk] = *reinterpret_cast<const at_bf16x8*>(tile + at(row0 + (lane & 31), 2 * kk + (lane >> 5)));
+    return f;
+  }
+  static __device__ __forceinline__ void rows(at_f32x16& acc, const Rows& f, const Own& o) {
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; kk++) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v[kk], o.v[kk], acc, 0, 0, 0);
+  }
+  // 32 rows of a tile as the operand of `cols`: a transposing read takes 4 rows x 16 dims per 16 lanes; lane
+  // i points at 4 dims of row i / 4 and gets dim i of the 4 rows
+  struct Cols {
+    union {
+      at_s16x4 h[2];
+      at_bf16x8 v;
+    } f[2][HD / 32];
+  };
+  static __device__ __forceinline__ Cols load_cols(const E* tile, int row0, int lane) {
+    Cols c;
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; dt++) {
+        const int row = row0 + 16 * kk + 4 * (lane >> 5) + ((lane >> 2) & 3);
+        const int dim = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          c.f[kk][dt].h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) at_s16x4*)(tile + at(row + 8 * j, dim >> 3) + (dim & 7)));
+      }
+    return c;
   }
   // w is rounded to bf16: the probabilities (or their gradients) enter a product as the tensors do
-  static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const E* tile, int row0, const at_f32x16& w,
-                                              int lane) {
+  static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const Cols& c, const at_f32x16& w, int) {
 #pragma unroll
     for (int kk = 0; kk < 2; kk++) {
       at_bf16x8 b;
 #pragma unroll
       for (int e = 0; e < 8; e++) b[e] = (__bf16)w[8 * kk + e];
-      // a transposing read takes 4 rows x 16 dims per 16 lanes: lane i points at 4 dims of row i / 4 and
-      // gets dim i of the 4 rows
-      const int row = row0 + 16 * kk + 4 * (lane >> 5) + ((lane >> 2) & 3);
 #pragma unroll
-      for (int dt = 0; dt < HD / 32; dt++) {
-        const int dim = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-        union {
-          at_s16x4 h[2];
-          at_bf16x8 v;
-        } a;
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          a.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) at_s16x4*)(tile + at(row + 8 * j, dim >> 3) + (dim & 7)));
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b, acc[dt], 0, 0, 0);
-      }
+      for (int dt = 0; dt < HD / 32; dt++)
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c.f[kk][dt].v, b, acc[dt], 0, 0, 0);
     }
   }
 };
@@ -161,22 +184,33 @@ struct AtMma<float, HD> {
     for (int i = 0; i < HD / 2; i++) s = fmaf(a.v[i], b.v[i], s);
     return s;
   }
-  static __device__ __forceinline__ void rows(at_f32x16& acc, const E* tile, int row0, const Own& o, int lane) {
-    const int row = row0 + (lane & 31);
+  // (an MFMA takes 64 cycles here and one or two LDS reads: they are read where they are used)
+  struct Rows {
+    const E* tile;
+    int row, half;
+  };
+  static __device__ __forceinline__ Rows load_rows(const E* tile, int row0, int lane) {
+    return {tile, row0 + (lane & 31), lane >> 5};
+  }
+  static __device__ __forceinline__ void rows(at_f32x16& acc, const Rows& f, const Own& o) {
 #pragma unroll
     for (int c = 0; c < HD / 8; c++) {
-      const float4 a = *reinterpret_cast<const float4*>(tile + at(row, (lane >> 5) * (HD / 8) + c));
+      const float4 a = *reinterpret_cast<const float4*>(f.tile + at(f.row, f.half * (HD / 8) + c));
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, o.v[4 * c], acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, o.v[4 * c + 1], acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, o.v[4 * c + 2], acc, 0, 0, 0);
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, o.v[4 * c + 3], acc, 0, 0, 0);
     }
   }
-  // row0 a multiple of 32: of a row's swizzle, bits 2 (HD 32) or 3 (`high`) and up are constants
-  static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const E* tile, int row0, const at_f32x16& w,
-                                              int lane) {
+  struct Cols {
+    const E* tile;
+  };
+  static __device__ __forceinline__ Cols load_cols(const E* tile, int row0, int) { return {tile + row0 * kStride}; }
+  // the tile's rows start at a multiple of 32: of a row's swizzle, bits 2 (HD 32) or 3 (`high`) and up are
+  // constants
+  static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const Cols& f, const at_f32x16& w, int lane) {
     const int half = lane >> 5, c = (lane & 31) >> 2;
-    const E* t = tile + (row0 + 4 * half) * kStride + (lane & 3);
+    const E* t = f.tile + 4 * half * kStride + (lane & 3);
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int row = (r >> 2) * 8 + (r & 3), high = (r >> 2) & 1;
@@ -217,89 +251,116 @@ __device__ __forceinline__ void at_fetch(E* tile, const AtRows<E>& m, int first,
   }
 }
 
-// This wave's requests have landed and its LDS reads are done; BLOCK: every wave's of the block.  (The
-// builtin, unlike a wait in inline assembly, also tells the compiler that nothing is in flight.)
-template <bool BLOCK>
-__device__ __forceinline__ void at_landed() {
+// Waits until at most VM of this wave's requests are on their way (and, VM < 0, no count is asked for) and
+// its LDS reads are done.  (The builtin, unlike a wait in inline assembly, also tells the compiler so.)
+template <int VM>
+__device__ __forceinline__ void at_wait() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-  if constexpr (BLOCK) __builtin_amdgcn_s_barrier();
+  constexpr int vm = VM < 0 || VM > 63 ? 63 : VM;
+  __builtin_amdgcn_s_waitcnt(0x0070 | (vm & 15) | (vm >> 4) << 14);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Every wave's requests have landed and every wave's LDS reads are done.
+__device__ __forceinline__ void at_landed() {
+  at_wait<0>();
+  __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// acc^T (dims x own rows) times f to row `row` (a pointer to its hd elements) of the lane's own row
-template <typename E, int HD, bool VEC>
-__device__ __forceinline__ void at_store(E* row, const at_f32x16 (&acc)[HD / 32], float f, int hd, int lane) {
+// acc^T (dims x own rows) times f to the 32 rows from `base` on (stride elements apart, hd of them each), of
+// which `rows` exist and the first `len` count: the others are zeros.  LDS: by whole 16-byte chunks of a
+// row through the wave's part of LDS, `tile` of 32 HD elements; the pieces that a lane holds (4 dims of
+// 32 different rows) would be partial writes of every line (dk and dv of 8 x 1024 rows: 42 us, 35 without
+// the stores).
+template <typename E, int HD, bool VEC, bool LDS>
+__device__ __forceinline__ void at_store(E* base, int stride, const at_f32x16 (&acc)[HD / 32], float f, int rows, int len,
+                                         int hd, E* tile, int lane) {
+  typedef AtMma<E, HD> M;
   typedef E e4 __attribute__((ext_vector_type(4)));
+  constexpr int CE = 16 / sizeof(E);
+  const int i = lane & 31;
 #pragma unroll
   for (int dt = 0; dt < HD / 32; dt++)
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       const int dim = dt * 32 + 8 * g + 4 * (lane >> 5);
-      const e4 v = {(E)(acc[dt][4 * g] * f), (E)(acc[dt][4 * g + 1] * f), (E)(acc[dt][4 * g + 2] * f),
-                    (E)(acc[dt][4 * g + 3] * f)};
-      if constexpr (VEC) {
-        if (dim < hd) *reinterpret_cast<e4*>(row + dim) = v;
+      e4 v = {(E)(acc[dt][4 * g] * f), (E)(acc[dt][4 * g + 1] * f), (E)(acc[dt][4 * g + 2] * f),
+              (E)(acc[dt][4 * g + 3] * f)};
+      if (i >= len) v = e4{(E)0.f, (E)0.f, (E)0.f, (E)0.f};
+      if constexpr (LDS) {
+        *reinterpret_cast<e4*>(tile + M::at(i, dim / CE) + dim % CE) = v;
+      } else if constexpr (VEC) {
+        if (i < rows && dim < hd) *reinterpret_cast<e4*>(base + (size_t)i * stride + dim) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (dim + e < hd) row[dim + e] = v[e];
+          if (i < rows && dim + e < hd) base[(size_t)i * stride + dim + e] = v[e];
       }
     }
+  if constexpr (LDS) {
+    constexpr int RP = 64 / M::kChunks;
+#pragma unroll
+    for (int p = 0; p < 32 / RP; p++) {
+      const int row = p * RP + lane / M::kChunks, c = lane % M::kChunks;
+      const at_u32x4 v = *reinterpret_cast<const at_u32x4*>(tile + M::at(row, c));
+      if (row < rows && c * CE < hd) *reinterpret_cast<at_u32x4*>(base + (size_t)row * stride + c * CE) = v;
+    }
+  }
 }
 
-// How a block goes through the axis it walks.  KS == 1: its four waves own 32 rows each of the other
-// axis and share tiles of kRows rows.  KS == 4: they own the same 32 rows and each walks every fourth
-// 32-row part through tiles of its own, without a barrier; their sums are joined at the end.
-// Tiles are requested one ahead into the other of two buffers (one buffer where two do not fit).
+// How a block goes through the axis it walks.
+// KS == 1: its four waves own 32 rows each of the other axis and share tiles of kRows rows, which are
+// requested one ahead into the other of two buffers (at_walk).
+// KS == 4: they own the same 32 rows; each takes every fourth 32-row part through tiles of its own,
+// without a barrier, and the sums are joined at the end.  A part's two tiles have one place each: the
+// next part's is requested as soon as a tile has been read for the last time, while the products with
+// the other one run, so that two blocks fit a CU.
 template <typename E, int HD, int KS, bool VEC>
 struct AtPlan {
   static constexpr int kOwn = 128 / KS;  // rows of a block
-  static constexpr int kRows = KS == 4 ? 128 : sizeof(E) == 4 && HD == 128 ? 32 : 64;
-  static constexpr int kParts = kRows / (32 * KS);     // 32-row parts of a wave
-  static constexpr int kTile = (KS == 4 ? 32 : kRows) * HD;  // elements of one operand's tile
-  static constexpr int kBufs = VEC && !(KS == 4 && sizeof(E) == 4 && HD == 128) ? 2 : 1;
+  static constexpr int kRows = KS == 4 ? 32 : sizeof(E) == 4 && HD == 128 ? 32 : 64;
+  static constexpr int kParts = kRows / 32;   // 32-row parts of a tile
+  static constexpr int kTile = kRows * HD;    // elements of one operand's tile
+  static constexpr int kLoads = kTile * (int)sizeof(E) / 1024 / (KS == 4 ? 1 : 4);  // a wave's requests for a tile
+  static constexpr int kBufs = VEC && KS == 1 ? 2 : 1;
   static constexpr int kBytes = 2 * kTile * KS * (int)sizeof(E);  // a buffer: both operands, all waves
+  static constexpr bool kStaged = VEC && KS == 1 && 128 * HD * (int)sizeof(E) <= kBytes;  // at_store's LDS fits one
 };
 
-// The tiles of two operands into `tiles` (the second kTile elements on): by all four waves of the
-// block (KS == 1), or by this wave alone.
+// A tile of the operand x: by all four waves of the block (KS == 1), or by this wave alone.
 template <typename E, int HD, int KS, bool VEC>
-__device__ __forceinline__ void at_load(E* tiles, const AtRows<E>& x, const AtRows<E>& y, int w, int lane) {
+__device__ __forceinline__ void at_load(E* tile, const AtRows<E>& x, int w, int lane) {
   typedef AtPlan<E, HD, KS, VEC> P;
-  if constexpr (VEC) {
-    constexpr int ROWS = KS == 4 ? 32 : P::kRows, WAVES = KS == 4 ? 1 : 4;
-    at_fetch<E, HD, ROWS, WAVES>(tiles, x, KS == 4 ? 0 : w, lane);
-    at_fetch<E, HD, ROWS, WAVES>(tiles + P::kTile, y, KS == 4 ? 0 : w, lane);
-  } else {
-    static_assert(KS == 1, "element loads are shared by the block");
-    at_stage<E, HD, P::kRows, false>(tiles, x, 64 * w + lane);
-    at_stage<E, HD, P::kRows, false>(tiles + P::kTile, y, 64 * w + lane);
-  }
+  static_assert(VEC || KS == 1, "element loads are shared by the block");
+  if constexpr (VEC)
+    at_fetch<E, HD, P::kRows, KS == 4 ? 1 : 4>(tile, x, KS == 4 ? 0 : w, lane);
+  else
+    at_stage<E, HD, P::kRows, false>(tile, x, 64 * w + lane);
 }
-// The steps 0 .. n - 1 of a walk: step kt computes on a buffer whose tiles have landed while those of
+// KS == 1: the steps 0 .. n - 1 of a walk: step kt computes on a buffer whose tiles have landed while those of
 // kt + 1 are on their way to the other.  The two buffers are LDS variables of their own and appear by
 // name in code of their own, so that the compiler does not make the reads of one wait for the other.
-template <typename P, int KS, typename F, typename C>
+template <typename P, typename F, typename C>
 __device__ __forceinline__ void at_walk(int n, char* even, char* odd, const F& fetch, const C& compute) {
   if constexpr (P::kBufs == 2) {
     fetch(0, even);
     for (int kt = 0; kt < n; kt += 2) {
-      at_landed<KS == 1>();
+      at_landed();
       if (kt + 1 < n) fetch(kt + 1, odd);
       compute(kt, even);
       if (kt + 1 == n) break;
-      at_landed<KS == 1>();
+      at_landed();
       if (kt + 2 < n) fetch(kt + 2, even);
       compute(kt + 1, odd);
     }
   } else {
     for (int kt = 0; kt < n; kt++) {
-      at_landed<KS == 1>();  // the last tile's reads are done
+      at_landed();  // the last tile's reads are done
       fetch(kt, even);
-      at_landed<KS == 1>();
+      at_landed();
       compute(kt, even);
     }
   }
@@ -307,17 +368,23 @@ __device__ __forceinline__ void at_walk(int n, char* even, char* odd, const F& f
 
 // Block -> (block of the axis, group = sequence * heads + head) of a causal launch over nblk * G
 // blocks; block 0 of the axis is the one with the most work, and is started first.  Workgroups reach
-// the 8 XCDs round-robin: when 8 divides G, an XCD takes whole neighbouring groups, so that what their
-// blocks share is fetched into its L2 only.
+// the 8 XCDs round-robin.  Sequences of one length: when 8 divides G, an XCD takes whole neighbouring
+// groups, so that what their blocks share is fetched into its L2 only; every other 32 of its blocks (one for
+// each of its CUs) come in reverse, so that a CU's blocks add up to the same (dq of 8 x 1024 rows, three
+// blocks to a CU: 32.1 -> 30.5 us).  Sequences of their own lengths:
+// a group's blocks go to all XCDs in turn, which evens out what long ones cost (4 x up to 1333 rows, 16
+// heads of 128, dq: 60 us with groups kept together, an XCD idle for half of it).
 struct AtBlock {
   int blk, g;
 };
-__device__ __forceinline__ AtBlock at_block(int L, int G) {
-  if (G % 8 == 0) {
-    const int s = L >> 3, gx = G / 8;
+__device__ __forceinline__ AtBlock at_block(int L, int G, int ragged) {
+  if (!ragged && G % 8 == 0) {
+    const int gx = G / 8, i = L >> 3, first = i & ~31, n = min(32, (int)(gridDim.x >> 3) - first);
+    const int s = i & 32 ? first + n - 1 - (i - first) : i;
     return {s / gx, (L & 7) * gx + s % gx};
   }
-  return {L / G, L % G};
+  const int blk = L / G, i = L % G;
+  return {blk, ragged && G % 2 == 0 ? (i + blk) % G : i};
 }
 
 __device__ __forceinline__ int at_len(const AttnTrain& a, int b) {

@@ -263,7 +263,8 @@ hipError_t launch_attn_forward(hipStream_t st, const AttnTrain& a, bool bf16, in
 hipError_t launch_attn_backward(hipStream_t st, const AttnTrain& a, bool bf16, int cus);
 
 // Distillation from a teacher's top logits (distill.hip): row losses, and gradients where dlogits is
-// not null (it may be logits); then their sum in double into acc[0] (added) or acc[1].
+// not null (it may be logits); then their sum in double into *sum (or added to it).  targets and sum may be
+// pinned host memory.
 constexpr int kDistillTop = 1024;
 struct DistillArgs {
   const void* logits;       // [T][V]
@@ -275,7 +276,7 @@ struct DistillArgs {
   int T, V, K, ignore;
   float tau, alpha, inv_count;
 };
-hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* acc, bool add);
+hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* sum, bool add);
 
 struct SampleArgs {
   const float* logits;  // [B][V] raw ForwardLast logits

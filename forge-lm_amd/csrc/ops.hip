@@ -1032,6 +1032,7 @@ struct OpsState {
   hipEvent_t stage_done[kStages] = {};
   int stage_next = 0;
   double* acc = nullptr;  // device loss accumulator + a result slot
+  double* result = nullptr;  // pinned host memory that a kernel writes a result to
   bool accumulating = false;
   long long accumulated_targets = 0;
 };
@@ -1043,6 +1044,7 @@ void ops_state_free(OpsState* o) {
   for (hipEvent_t e : o->stage_done)
     if (e) (void)hipEventDestroy(e);
   if (o->stage) (void)hipHostFree(o->stage);
+  if (o->result) (void)hipHostFree(o->result);
   delete o;
 }
 
@@ -1130,14 +1132,8 @@ int op_launched(const char* what) {
 // copied into the next staging area (16 KB of targets or ids in a microsecond), whose event
 // bounds how far the host runs ahead: waiting for each copy cost a training step 20-30 us per
 // upload with the device idle.
-int copy_ints(fh_context* c, OpsState* o, const int32_t* host, size_t n, int* dev) {
-  hipStream_t st = context_stream(c);
-  const size_t bytes = n * sizeof(int32_t);
-  if (bytes > kStageBytes) {
-    HIP_TRY(hipMemcpyAsync(dev, host, bytes, hipMemcpyHostToDevice, st));
-    HIP_TRY(hipStreamSynchronize(st));
-    return FH_OK;
-  }
+// n ints (at most kStageBytes) in the next staging area, *area; area_used says that the work that reads it is enqueued
+int stage_ints(OpsState* o, const int32_t* host, size_t n, const int** area) {
   if (!o->stage) {
     void* p = nullptr;
     HIP_TRY(hipHostMalloc(&p, kStages * kStageBytes, hipHostMallocDefault));
@@ -1148,12 +1144,29 @@ int copy_ints(fh_context* c, OpsState* o, const int32_t* host, size_t n, int* de
     HIP_TRY(hipEventSynchronize(o->stage_done[k]));
   else
     HIP_TRY(hipEventCreateWithFlags(&o->stage_done[k], hipEventDisableTiming));
-  char* from = o->stage + k * kStageBytes;
-  std::memcpy(from, host, bytes);
-  HIP_TRY(hipMemcpyAsync(dev, from, bytes, hipMemcpyHostToDevice, st));
-  HIP_TRY(hipEventRecord(o->stage_done[k], st));
-  o->stage_next = (k + 1) % kStages;
+  char* at = o->stage + k * kStageBytes;
+  std::memcpy(at, host, n * sizeof(int32_t));
+  *area = reinterpret_cast<const int*>(at);
   return FH_OK;
+}
+int area_used(fh_context* c, OpsState* o) {
+  HIP_TRY(hipEventRecord(o->stage_done[o->stage_next], context_stream(c)));
+  o->stage_next = (o->stage_next + 1) % kStages;
+  return FH_OK;
+}
+
+int copy_ints(fh_context* c, OpsState* o, const int32_t* host, size_t n, int* dev) {
+  hipStream_t st = context_stream(c);
+  const size_t bytes = n * sizeof(int32_t);
+  if (bytes > kStageBytes) {
+    HIP_TRY(hipMemcpyAsync(dev, host, bytes, hipMemcpyHostToDevice, st));
+    HIP_TRY(hipStreamSynchronize(st));
+    return FH_OK;
+  }
+  const int* from = nullptr;
+  FH_TRY(stage_ints(o, host, n, &from));
+  HIP_TRY(hipMemcpyAsync(dev, from, bytes, hipMemcpyHostToDevice, st));
+  return area_used(c, o);
 }
 
 int upload_ints(fh_context* c, OpsState* o, const int32_t* host, size_t n, int** dev) {
@@ -1162,6 +1175,9 @@ int upload_ints(fh_context* c, OpsState* o, const int32_t* host, size_t n, int**
   *dev = static_cast<int*>(p);
   return copy_ints(c, o, host, n, *dev);
 }
+
+// as many targets as blocks read from host memory themselves (fh_op_distill_loss)
+constexpr int kStagedTargets = 2048;
 
 // the partial sums of a split K take at most this much of the context's scratch (64 MB)
 constexpr size_t kSplitPartFloats = (size_t)16 << 20;
@@ -1796,23 +1812,35 @@ int fh_op_distill_loss(fh_context* c, const void* logits, const int32_t* targets
   OPS_PROLOGUE(c);
   void* p = nullptr;
   FH_TRY(ops_scratch(c, ops_, (size_t)T * (sizeof(int32_t) + sizeof(float)), &p));
-  int* dt = static_cast<int*>(p);
-  FH_TRY(copy_ints(c, ops_, targets, (size_t)T, dt));
+  if (!ops_->result) {
+    void* r = nullptr;
+    HIP_TRY(hipHostMalloc(&r, sizeof(double), hipHostMallocDefault));
+    ops_->result = static_cast<double*>(r);
+  }
   DistillArgs a{};
-  a.logits = logits, a.dlogits = dlogits, a.targets = dt, a.top_ids = top_ids_dev, a.top_logits = top_logits_dev;
-  a.row_loss = reinterpret_cast<float*>(dt + T);
+  a.logits = logits, a.dlogits = dlogits, a.top_ids = top_ids_dev, a.top_logits = top_logits_dev;
+  a.row_loss = static_cast<float*>(p) + T;
   a.T = T, a.V = V, a.K = K, a.ignore = ignore_index, a.tau = temperature, a.alpha = alpha;
   a.inv_count = count ? 1.f / (float)count : 0.f;
-  HIP_TRY(launch_distill(st_, a, dtype == FH_DTYPE_BF16, ops_->acc, ops_->accumulating));
+  // few targets: each row's block reads its own from the staging area, which costs a row some latency
+  // and saves a copy before the kernel
+  const bool staged = T <= kStagedTargets;
+  if (staged) {
+    FH_TRY(stage_ints(ops_, targets, (size_t)T, &a.targets));
+  } else {
+    FH_TRY(copy_ints(c, ops_, targets, (size_t)T, static_cast<int*>(p)));
+    a.targets = static_cast<const int*>(p);
+  }
+  const bool later = ops_->accumulating;  // the loss stays on the device until the accumulation ends
+  HIP_TRY(launch_distill(st_, a, dtype == FH_DTYPE_BF16, later ? ops_->acc : ops_->result, later));
+  if (staged) FH_TRY(area_used(c, ops_));
   *loss = 0.f;
-  if (ops_->accumulating) {  // the loss stays on the device until the accumulation ends
+  if (later) {
     ops_->accumulated_targets += count;
     return FH_OK;
   }
-  double sum = 0;
-  HIP_TRY(hipMemcpyAsync(&sum, ops_->acc + 1, sizeof(double), hipMemcpyDeviceToHost, st_));
   HIP_TRY(hipStreamSynchronize(st_));
-  if (count) *loss = (float)(sum / count);
+  if (count) *loss = (float)(*ops_->result / count);
   return FH_OK;
 }
 
