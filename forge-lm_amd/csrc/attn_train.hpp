@@ -7,8 +7,10 @@
 //                                                   register r, tile row (r/4)*8 + (l/32)*4 + r%4
 //   cols  acc[d][i] += sum_r tile[r][d] w[r][i]     the score registers are the B operand as they
 //                                                   are; the tile is read transposed
-// fp32 tensors multiply on v_mfma_f32_32x32x2_f32 (exact fp32 products and sums), bf16 ones on
-// v_mfma_f32_32x32x16_bf16 with fp32 sums; softmax statistics and sums are fp32 in both.
+// bf16 tensors multiply on v_mfma_f32_32x32x16_bf16, fp32 ones on v_mfma_f32_32x32x2_f32 (exact products)
+// or, where that pays (attn_train_split), as three bf16 parts each on the former: a = hi + mid + lo holds
+// all 24 bits, and the six products down to 2^-16 of the largest leave out what is below 2^-24 of it, at
+// 6 x 32 cycles for 16 dims where the fp32 instruction takes 8 x 64.  Sums and softmax statistics are fp32.
 #pragma once
 
 #include "kernels.hpp"
@@ -24,6 +26,22 @@ typedef short at_s16x4 __attribute__((ext_vector_type(4)));
 
 template <int I>
 constexpr std::integral_constant<int, I> at_int{};
+
+// What a kernel computes on: the element of its tiles, that of the tensors it writes, and the parts that a
+// value is held in.
+struct AtF32 {
+  typedef float E, O;
+  static constexpr int kParts = 1;
+};
+struct AtBf16 {
+  typedef __bf16 E, O;
+  static constexpr int kParts = 1;
+};
+struct AtSplit {
+  typedef __bf16 E;
+  typedef float O;
+  static constexpr int kParts = 3;
+};
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -67,187 +85,226 @@ __device__ __forceinline__ at_u32x4 at_chunk(const AtRows<E>& m, int row, int ch
   }
 }
 
-// The two products and the operand layouts of a type, for heads padded to HD.
+// LDS rows of HD elements in 16-byte chunks, permuted by row.
 template <typename E, int HD>
-struct AtMma;
-
+struct AtTile;
 template <int HD>
-struct AtMma<__bf16, HD> {
-  typedef __bf16 E;
-  static constexpr int kChunks = HD / 8;  // 16-byte chunks of a row
-  static constexpr int kStride = HD;      // LDS elements of a row
-  // Chunks of a row are permuted so that the 16 lanes of a 16-byte read (16 rows, one chunk) and the
-  // 32 of a transposing read (4 rows, 64 bytes of each) fall on distinct banks.
+struct AtTile<__bf16, HD> {
+  static constexpr int kChunks = HD / 8;
+  // the 16 lanes of a 16-byte read (16 rows, one chunk) and the 32 of a transposing read (4 rows, 64 bytes of
+  // each) fall on distinct banks
   static __device__ __forceinline__ int swizzle(int row) {
     if constexpr (HD == 32) return (row >> 2) & 3;
     if constexpr (HD == 64) return ((row & 2) << 1) | ((row & 4) >> 1) | ((row >> 3) & 1);
     return ((row & 3) << 2) | ((row & 4) >> 1) | ((row >> 3) & 1);
   }
-  static __device__ __forceinline__ int at(int row, int chunk) { return row * kStride + 8 * (chunk ^ swizzle(row)); }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * HD + 8 * (chunk ^ swizzle(row)); }
+};
+template <int HD>
+struct AtTile<float, HD> {
+  static constexpr int kChunks = HD / 4;
+  // 16 rows of one chunk on distinct banks; the 32 lanes of a column read share a row
+  static __device__ __forceinline__ int swizzle(int row) { return HD == 32 ? (row >> 1) & 7 : row & 15; }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * HD + 4 * (chunk ^ swizzle(row)); }
+};
+
+// The two products, for heads padded to HD.  A tile of a kind in parts is its parts' tiles, `part` elements
+// apart.
+template <typename K, int HD>
+struct AtMma {
+  typedef __bf16 E;
+  typedef AtTile<E, HD> L;
+  static constexpr int N = K::kParts;
   struct Own {
-    at_bf16x8 v[HD / 16];  // own row l % 32, dims 16 kk + 8 (l / 32) ..
+    at_bf16x8 v[N][HD / 16];  // own row l % 32, dims 16 kk + 8 (l / 32) ..
   };
   template <bool VEC>
-  static __device__ __forceinline__ Own own(const AtRows<E>& m, int row, int lane) {
-    Own o;
+  static __device__ __forceinline__ void own(at_bf16x8 (&v)[HD / 16], const AtRows<E>& m, int lane) {
 #pragma unroll
     for (int kk = 0; kk < HD / 16; kk++)
-      o.v[kk] = __builtin_bit_cast(at_bf16x8, at_chunk<E, VEC>(m, row, 2 * kk + (lane >> 5)));
-    return o;
+      v[kk] = __builtin_bit_cast(at_bf16x8, at_chunk<E, VEC>(m, lane & 31, 2 * kk + (lane >> 5)));
   }
   // a lane's half of the dot product of two own rows
-  static __device__ __forceinline__ float dot(const Own& a, const Own& b) {
+  static __device__ __forceinline__ float dot(const at_bf16x8 (&a)[HD / 16], const at_bf16x8 (&b)[HD / 16]) {
     float s = 0.f;
 #pragma unroll
     for (int kk = 0; kk < HD / 16; kk++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) s = fmaf((float)a.v[kk][e], (float)b.v[kk][e], s);
+      for (int e = 0; e < 8; e++) s = fmaf((float)a[kk][e], (float)b[kk][e], s);
     return s;
   }
-  // 32 rows of a tile as the operand of `rows`
-  struct Rows {
-    at_bf16x8 v[HD / 16];
-  };
-  static __device__ __forceinline__ Rows load_rows(const E* tile, int row0, int lane) {
-    Rows f;
+  // acc += the products of parts a_i b_j, i + j < N, the small ones first
+  static __device__ __forceinline__ void mul(at_f32x16& acc, const at_bf16x8 (&a)[N], const at_bf16x8 (&b)[N]) {
 #pragma unroll
-    for (int kk = 0; kk < HD / 16; kk++)
-      f.v[kk] = *reinterpret_cast<const at_bf16x8*>(tile + at(row0 + (lane & 31), 2 * kk + (lane >> 5)));
-    return f;
+    for (int sum = N - 1; sum >= 0; sum--)
+#pragma unroll
+      for (int i = 0; i <= sum; i++) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[sum - i], acc, 0, 0, 0);
   }
-  static __device__ __forceinline__ void rows(at_f32x16& acc, const Rows& f, const Own& o) {
+  static __device__ __forceinline__ void rows(at_f32x16& acc, const E* tile, int part, int row0, const Own& o, int lane) {
 #pragma unroll
-    for (int kk = 0; kk < HD / 16; kk++) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v[kk], o.v[kk], acc, 0, 0, 0);
+    for (int kk = 0; kk < HD / 16; kk++) {
+      at_bf16x8 a[N], b[N];
+#pragma unroll
+      for (int p = 0; p < N; p++) {
+        a[p] = *reinterpret_cast<const at_bf16x8*>(tile + p * part + L::at(row0 + (lane & 31), 2 * kk + (lane >> 5)));
+        b[p] = o.v[p][kk];
+      }
+      mul(acc, a, b);
+    }
   }
   // 32 rows of a tile as the operand of `cols`: a transposing read takes 4 rows x 16 dims per 16 lanes; lane
   // i points at 4 dims of row i / 4 and gets dim i of the 4 rows
-  struct Cols {
+  static __device__ __forceinline__ at_bf16x8 column(const E* tile, int row0, int kk, int dt, int lane) {
+    const int row = row0 + 16 * kk + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int dim = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     union {
       at_s16x4 h[2];
       at_bf16x8 v;
-    } f[2][HD / 32];
+    } f;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+      f.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) at_s16x4*)(tile + L::at(row + 8 * j, dim >> 3) + (dim & 7)));
+    return f.v;
+  }
+  static constexpr bool kAhead = N == 1 && HD <= 64;  // registers for it before the exponentials
+  struct Cols {
+    const E* tile;
+    int part, row0;
+    at_bf16x8 f[kAhead ? 2 : 1][HD / 32];
   };
-  static __device__ __forceinline__ Cols load_cols(const E* tile, int row0, int lane) {
+  static __device__ __forceinline__ Cols load_cols(const E* tile, int part, int row0, int lane) {
     Cols c;
+    c.tile = tile, c.part = part, c.row0 = row0;
+    if constexpr (kAhead)
 #pragma unroll
-    for (int kk = 0; kk < 2; kk++)
+      for (int kk = 0; kk < 2; kk++)
 #pragma unroll
-      for (int dt = 0; dt < HD / 32; dt++) {
-        const int row = row0 + 16 * kk + 4 * (lane >> 5) + ((lane >> 2) & 3);
-        const int dim = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          c.f[kk][dt].h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) at_s16x4*)(tile + at(row + 8 * j, dim >> 3) + (dim & 7)));
-      }
+        for (int dt = 0; dt < HD / 32; dt++) c.f[kk][dt] = column(tile, row0, kk, dt, lane);
     return c;
   }
-  // w is rounded to bf16: the probabilities (or their gradients) enter a product as the tensors do
-  static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const Cols& c, const at_f32x16& w, int) {
+  // w enters a product as the tensors do: rounded to bf16, or in three parts
+  static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const Cols& c, const at_f32x16& w, int lane) {
 #pragma unroll
     for (int kk = 0; kk < 2; kk++) {
-      at_bf16x8 b;
+      at_bf16x8 b[N];
 #pragma unroll
-      for (int e = 0; e < 8; e++) b[e] = (__bf16)w[8 * kk + e];
+      for (int e = 0; e < 8; e++) {
+        float x = w[8 * kk + e];
 #pragma unroll
-      for (int dt = 0; dt < HD / 32; dt++)
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c.f[kk][dt].v, b, acc[dt], 0, 0, 0);
+        for (int p = 0; p < N; p++) {
+          b[p][e] = (__bf16)x;
+          if (p + 1 < N) x -= (float)b[p][e];
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; dt++) {
+        at_bf16x8 a[N];
+#pragma unroll
+        for (int p = 0; p < N; p++) a[p] = kAhead ? c.f[kAhead ? kk : 0][dt] : column(c.tile + p * c.part, c.row0, kk, dt, lane);
+        mul(acc[dt], a, b);
+      }
     }
   }
 };
 
 template <int HD>
-struct AtMma<float, HD> {
+struct AtMma<AtF32, HD> {
   typedef float E;
-  static constexpr int kChunks = HD / 4;
-  static constexpr int kStride = HD;
-  // 16 rows of one chunk on distinct banks; the 32 lanes of a column read share a row
-  static __device__ __forceinline__ int swizzle(int row) { return HD == 32 ? (row >> 1) & 7 : row & 15; }
-  static __device__ __forceinline__ int at(int row, int chunk) { return row * kStride + 4 * (chunk ^ swizzle(row)); }
+  typedef AtTile<E, HD> L;
   struct Own {
-    float v[HD / 2];  // own row l % 32, dims (l / 32) HD / 2 ..: a product step pairs dims d and d + HD / 2
+    float v[1][HD / 2];  // own row l % 32, dims (l / 32) HD / 2 ..: a product step pairs dims d and d + HD / 2
   };
   template <bool VEC>
-  static __device__ __forceinline__ Own own(const AtRows<E>& m, int row, int lane) {
-    Own o;
+  static __device__ __forceinline__ void own(float (&v)[HD / 2], const AtRows<E>& m, int lane) {
 #pragma unroll
     for (int c = 0; c < HD / 8; c++) {
-      const at_u32x4 x = at_chunk<E, VEC>(m, row, (lane >> 5) * (HD / 8) + c);
+      const at_u32x4 x = at_chunk<E, VEC>(m, lane & 31, (lane >> 5) * (HD / 8) + c);
 #pragma unroll
-      for (int e = 0; e < 4; e++) o.v[4 * c + e] = __uint_as_float(x[e]);
+      for (int e = 0; e < 4; e++) v[4 * c + e] = __uint_as_float(x[e]);
     }
-    return o;
   }
-  static __device__ __forceinline__ float dot(const Own& a, const Own& b) {
+  static __device__ __forceinline__ float dot(const float (&a)[HD / 2], const float (&b)[HD / 2]) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD / 2; i++) s = fmaf(a.v[i], b.v[i], s);
+    for (int i = 0; i < HD / 2; i++) s = fmaf(a[i], b[i], s);
     return s;
   }
-  // (an MFMA takes 64 cycles here and one or two LDS reads: they are read where they are used)
-  struct Rows {
-    const E* tile;
-    int row, half;
-  };
-  static __device__ __forceinline__ Rows load_rows(const E* tile, int row0, int lane) {
-    return {tile, row0 + (lane & 31), lane >> 5};
-  }
-  static __device__ __forceinline__ void rows(at_f32x16& acc, const Rows& f, const Own& o) {
+  static __device__ __forceinline__ void rows(at_f32x16& acc, const E* tile, int, int row0, const Own& o, int lane) {
 #pragma unroll
     for (int c = 0; c < HD / 8; c++) {
-      const float4 a = *reinterpret_cast<const float4*>(f.tile + at(f.row, f.half * (HD / 8) + c));
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, o.v[4 * c], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, o.v[4 * c + 1], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, o.v[4 * c + 2], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, o.v[4 * c + 3], acc, 0, 0, 0);
+      const float4 a = *reinterpret_cast<const float4*>(tile + L::at(row0 + (lane & 31), (lane >> 5) * (HD / 8) + c));
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, o.v[0][4 * c], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, o.v[0][4 * c + 1], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, o.v[0][4 * c + 2], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, o.v[0][4 * c + 3], acc, 0, 0, 0);
     }
   }
+  static constexpr bool kAhead = false;  // (an MFMA takes 64 cycles here and one LDS read)
   struct Cols {
     const E* tile;
   };
-  static __device__ __forceinline__ Cols load_cols(const E* tile, int row0, int) { return {tile + row0 * kStride}; }
+  static __device__ __forceinline__ Cols load_cols(const E* tile, int, int row0, int) { return {tile + row0 * HD}; }
   // the tile's rows start at a multiple of 32: of a row's swizzle, bits 2 (HD 32) or 3 (`high`) and up are
   // constants
   static __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const Cols& f, const at_f32x16& w, int lane) {
     const int half = lane >> 5, c = (lane & 31) >> 2;
-    const E* t = f.tile + 4 * half * kStride + (lane & 3);
+    const E* t = f.tile + 4 * half * HD + (lane & 3);
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int row = (r >> 2) * 8 + (r & 3), high = (r >> 2) & 1;
       const int low = HD == 32 ? (c ^ (2 * half + ((r & 3) >> 1))) ^ (4 * high) : c ^ (4 * half + (r & 3));
 #pragma unroll
       for (int dt = 0; dt < HD / 32; dt++)
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(t[row * kStride + 4 * low + (HD == 32 ? 0 : 32 * (dt ^ high))], w[r],
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(t[row * HD + 4 * low + (HD == 32 ? 0 : 32 * (dt ^ high))], w[r],
                                                        acc[dt], 0, 0, 0);
     }
   }
 };
 
-// SR rows of m into an LDS tile, by the block's 256 threads.
-template <typename E, int HD, int SR, bool VEC>
-__device__ __forceinline__ void at_stage(E* tile, const AtRows<E>& m, int tid) {
-  typedef AtMma<E, HD> M;
+// A matrix in parts: the rows of each, `part` elements (of the whole matrix) apart.
+template <typename K>
+struct AtSource {
+  const typename K::E* base;
+  size_t part;
+  int stride, hd;  // elements of a row and of a head
+  __device__ __forceinline__ AtRows<typename K::E> rows(int p, size_t row, size_t col, int n) const {
+    return at_rows(base + p * part + row * stride + col, n, stride, hd);
+  }
+};
+template <typename K, int HD, bool VEC>
+__device__ __forceinline__ void at_own(typename AtMma<K, HD>::Own& o, const AtSource<K>& x, size_t row, size_t col, int rows,
+                                       int lane) {
 #pragma unroll
-  for (int i = 0; i < SR * M::kChunks / 256; i++) {
-    const int row = (tid + 256 * i) / M::kChunks, c = (tid + 256 * i) % M::kChunks;
-    *reinterpret_cast<at_u32x4*>(tile + M::at(row, c)) = at_chunk<E, VEC>(m, row, c);
+  for (int p = 0; p < K::kParts; p++) AtMma<K, HD>::template own<VEC>(o.v[p], x.rows(p, row, col, rows), lane);
+}
+
+// SR rows of m into an LDS tile, by the block's 256 threads.
+template <int HD, int SR, bool VEC, typename E>
+__device__ __forceinline__ void at_stage(E* tile, const AtRows<E>& m, int tid) {
+  typedef AtTile<E, HD> L;
+#pragma unroll
+  for (int i = 0; i < SR * L::kChunks / 256; i++) {
+    const int row = (tid + 256 * i) / L::kChunks, c = (tid + 256 * i) % L::kChunks;
+    *reinterpret_cast<at_u32x4*>(tile + L::at(row, c)) = at_chunk<E, VEC>(m, row, c);
   }
 }
 
 // ROWS rows of m straight into an LDS tile: 1 KB pieces (64 lanes x 16 bytes, contiguous in LDS),
 // every WAVES-th of them from `first` by this wave.  A lane asks for the chunk whose place is its own.
 // Chunks past either end of m arrive as zeros.
-template <typename E, int HD, int ROWS, int WAVES>
-__device__ __forceinline__ void at_fetch(E* tile, const AtRows<E>& m, int first, int lane) {
-  typedef AtMma<E, HD> M;
-  constexpr int CE = 16 / sizeof(E), RP = 64 / M::kChunks, N = ROWS / RP / WAVES;
-  static_assert(N * RP * WAVES == ROWS, "pieces");
+template <typename K, int HD, int ROWS, int WAVES>
+__device__ __forceinline__ void at_fetch(typename K::E* tile, const AtRows<typename K::E>& m, int first, int lane) {
+  typedef typename K::E E;
+  typedef AtTile<E, HD> L;
+  constexpr int CE = 16 / sizeof(E), RP = 64 / L::kChunks, N = (ROWS / RP + WAVES - 1) / WAVES;
 #pragma unroll
   for (int i = 0; i < N; i++) {
-    const int row0 = (first + WAVES * i) * RP, row = row0 + lane / M::kChunks;
-    const int c = (lane % M::kChunks) ^ M::swizzle(row);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(m.rsrc, (__attribute__((address_space(3))) void*)(tile + row0 * M::kStride), 16,
-                                             c * CE < m.hd ? row * m.stride + c * 16 : 0x7ffffff0, 0, 0, 0);
+    const int row0 = (first + WAVES * i) * RP, row = row0 + lane / L::kChunks;
+    const int c = (lane % L::kChunks) ^ L::swizzle(row);
+    if (ROWS / RP % WAVES == 0 || first + WAVES * i < ROWS / RP)  // (fewer pieces than waves)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(m.rsrc, (__attribute__((address_space(3))) void*)(tile + row0 * HD), 16,
+                                               c * CE < m.hd ? row * m.stride + c * 16 : 0x7ffffff0, 0, 0, 0);
   }
 }
 
@@ -271,43 +328,53 @@ __device__ __forceinline__ void at_landed() {
 }
 
 // acc^T (dims x own rows) times f to the 32 rows from `base` on (stride elements apart, hd of them each), of
-// which `rows` exist and the first `len` count: the others are zeros.  LDS: by whole 16-byte chunks of a
-// row through the wave's part of LDS, `tile` of 32 HD elements; the pieces that a lane holds (4 dims of
-// 32 different rows) would be partial writes of every line (dk and dv of 8 x 1024 rows: 42 us, 35 without
-// the stores).
-template <typename E, int HD, bool VEC, bool LDS>
-__device__ __forceinline__ void at_store(E* base, int stride, const at_f32x16 (&acc)[HD / 32], float f, int rows, int len,
-                                         int hd, E* tile, int lane) {
-  typedef AtMma<E, HD> M;
-  typedef E e4 __attribute__((ext_vector_type(4)));
-  constexpr int CE = 16 / sizeof(E);
+// which `rows` exist and the first `len` count: the others are zeros.  RPP > 0: RPP rows at a time by whole
+// 16-byte chunks of a row through the wave's part of LDS, `tile` of RPP * HD elements; the pieces that a lane
+// holds (4 dims of 32 different rows) would be partial writes of every line (dk and dv of 8 x 1024 bf16 rows:
+// 42 us, 35 without the stores).  RPP 0: by the pieces, VEC, or by elements.
+template <typename O, int HD, bool VEC, int RPP>
+__device__ __forceinline__ void at_store(O* base, int stride, const at_f32x16 (&acc)[HD / 32], float f, int rows, int len,
+                                         int hd, O* tile, int lane) {
+  typedef AtTile<O, HD> L;
+  typedef O o4 __attribute__((ext_vector_type(4)));
+  constexpr int CE = 16 / sizeof(O);
   const int i = lane & 31;
+  auto each = [&](auto&& put) {
 #pragma unroll
-  for (int dt = 0; dt < HD / 32; dt++)
+    for (int dt = 0; dt < HD / 32; dt++)
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int dim = dt * 32 + 8 * g + 4 * (lane >> 5);
-      e4 v = {(E)(acc[dt][4 * g] * f), (E)(acc[dt][4 * g + 1] * f), (E)(acc[dt][4 * g + 2] * f),
-              (E)(acc[dt][4 * g + 3] * f)};
-      if (i >= len) v = e4{(E)0.f, (E)0.f, (E)0.f, (E)0.f};
-      if constexpr (LDS) {
-        *reinterpret_cast<e4*>(tile + M::at(i, dim / CE) + dim % CE) = v;
-      } else if constexpr (VEC) {
-        if (i < rows && dim < hd) *reinterpret_cast<e4*>(base + (size_t)i * stride + dim) = v;
+      for (int g = 0; g < 4; g++) {
+        const int dim = dt * 32 + 8 * g + 4 * (lane >> 5);
+        o4 v = {(O)(acc[dt][4 * g] * f), (O)(acc[dt][4 * g + 1] * f), (O)(acc[dt][4 * g + 2] * f),
+                (O)(acc[dt][4 * g + 3] * f)};
+        if (i >= len) v = o4{(O)0.f, (O)0.f, (O)0.f, (O)0.f};
+        put(dim, v);
+      }
+  };
+  if constexpr (RPP > 0) {
+    constexpr int RP = 64 / L::kChunks;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += RPP) {
+      if (RPP == 32 || (i >= r0 && i < r0 + RPP))
+        each([&](int dim, const o4& v) { *reinterpret_cast<o4*>(tile + L::at(i - r0, dim / CE) + dim % CE) = v; });
+#pragma unroll
+      for (int p = 0; p < RPP / RP; p++) {
+        const int row = p * RP + lane / L::kChunks, c = lane % L::kChunks;
+        const at_u32x4 v = *reinterpret_cast<const at_u32x4*>(tile + L::at(row, c));
+        if (r0 + row < rows && c * CE < hd) *reinterpret_cast<at_u32x4*>(base + (size_t)(r0 + row) * stride + c * CE) = v;
+      }
+    }
+  } else {
+    each([&](int dim, const o4& v) {
+      O* to = base + (size_t)i * stride + dim;
+      if constexpr (VEC) {
+        if (i < rows && dim < hd) *reinterpret_cast<o4*>(to) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (i < rows && dim + e < hd) base[(size_t)i * stride + dim + e] = v[e];
+          if (i < rows && dim + e < hd) to[e] = v[e];
       }
-    }
-  if constexpr (LDS) {
-    constexpr int RP = 64 / M::kChunks;
-#pragma unroll
-    for (int p = 0; p < 32 / RP; p++) {
-      const int row = p * RP + lane / M::kChunks, c = lane % M::kChunks;
-      const at_u32x4 v = *reinterpret_cast<const at_u32x4*>(tile + M::at(row, c));
-      if (row < rows && c * CE < hd) *reinterpret_cast<at_u32x4*>(base + (size_t)row * stride + c * CE) = v;
-    }
+    });
   }
 }
 
@@ -318,28 +385,54 @@ __device__ __forceinline__ void at_store(E* base, int stride, const at_f32x16 (&
 // without a barrier, and the sums are joined at the end.  A part's two tiles have one place each: the
 // next part's is requested as soon as a tile has been read for the last time, while the products with
 // the other one run, so that two blocks fit a CU.
-template <typename E, int HD, int KS, bool VEC>
+// VEC: rows of 16-byte chunks.
+template <typename K, int HD, int KS, bool VEC>
 struct AtPlan {
+  typedef typename K::E E;
+  typedef typename K::O O;
   static constexpr int kOwn = 128 / KS;  // rows of a block
-  static constexpr int kRows = KS == 4 ? 32 : sizeof(E) == 4 && HD == 128 ? 32 : 64;
-  static constexpr int kParts = kRows / 32;   // 32-row parts of a tile
-  static constexpr int kTile = kRows * HD;    // elements of one operand's tile
+  static constexpr int kRows = KS == 4 || K::kParts > 1 || sizeof(E) * HD > 256 ? 32 : 64;
+  static constexpr int kParts = kRows / 32;             // 32-row parts of a tile
+  static constexpr int kSub = kRows * HD;               // elements of one part of the values
+  static constexpr int kTile = kSub * K::kParts;        // elements of one operand's tile
   static constexpr int kLoads = kTile * (int)sizeof(E) / 1024 / (KS == 4 ? 1 : 4);  // a wave's requests for a tile
   static constexpr int kBufs = VEC && KS == 1 ? 2 : 1;
   static constexpr int kBytes = 2 * kTile * KS * (int)sizeof(E);  // a buffer: both operands, all waves
-  static constexpr bool kStaged = VEC && KS == 1 && 128 * HD * (int)sizeof(E) <= kBytes;  // at_store's LDS fits one
+  // at_store's rows at a time
+  static constexpr int kOut = !VEC || KS != 1 ? 0 : 128 * HD * (int)sizeof(O) <= kBytes ? 32
+                              : 64 * HD * (int)sizeof(O) <= kBytes ? 16 : 0;
 };
 
-// A tile of the operand x: by all four waves of the block (KS == 1), or by this wave alone.
-template <typename E, int HD, int KS, bool VEC>
-__device__ __forceinline__ void at_load(E* tile, const AtRows<E>& x, int w, int lane) {
-  typedef AtPlan<E, HD, KS, VEC> P;
-  static_assert(VEC || KS == 1, "element loads are shared by the block");
-  if constexpr (VEC)
-    at_fetch<E, HD, P::kRows, KS == 4 ? 1 : 4>(tile, x, KS == 4 ? 0 : w, lane);
-  else
-    at_stage<E, HD, P::kRows, false>(tile, x, 64 * w + lane);
+// Whether `blocks` blocks of 128 rows are so few that KS 4 pays: a wave's chain of steps is a quarter as long,
+// and every tile is fetched for 32 rows instead of 128.  us with KS 1 and KS 4, 12 heads of 64 but where said:
+//   bf16 forward   192 blocks (2 x 1024) 20 and 16, 256 (4 x 1024, 8 heads) 21 and 23, 384 (4 x 1024) 24 and 29
+//   bf16 backward  192 blocks 48 and 38, 384 57 and 67, 768 (8 x 1024) 77 and 129
+//   fp32 forward   192 blocks 87 and 53, 384 100 and 89, 768 153 and 165; heads of 128: 256 blocks (2 x 2000,
+//                  8 heads) 291 and 228, 384 (8 x 300, 16 heads) 73 and 98
+//   fp32 backward  96 blocks (2 x 512) 132 and 60, 288 (8 x 333, heads of 40) 118 and 99
+//   in parts, backward  192 blocks 175 and 144, 384 210 and 260
+template <typename K, int HD>
+bool at_few(size_t blocks, int cus) {
+  const size_t quarters = std::is_same_v<K, AtF32> ? HD > 64 ? 5 : 8 : 4;  // of the CUs
+  return 4 * blocks < quarters * cus;
 }
+
+// A tile of rows `row` .. of x: by all four waves of the block (KS == 1), or by this wave alone.
+template <typename K, int HD, int KS, bool VEC>
+__device__ __forceinline__ void at_load(typename K::E* tile, const AtSource<K>& x, size_t row, size_t col, int rows, int w,
+                                        int lane) {
+  typedef AtPlan<K, HD, KS, VEC> P;
+  static_assert(VEC || KS == 1, "element loads are shared by the block");
+#pragma unroll
+  for (int p = 0; p < K::kParts; p++) {
+    const AtRows<typename K::E> m = x.rows(p, row, col, min(rows, P::kRows));
+    if constexpr (VEC)
+      at_fetch<K, HD, P::kRows, KS == 4 ? 1 : 4>(tile + p * P::kSub, m, KS == 4 ? 0 : w, lane);
+    else
+      at_stage<HD, P::kRows, false>(tile + p * P::kSub, m, 64 * w + lane);
+  }
+}
+
 // KS == 1: the steps 0 .. n - 1 of a walk: step kt computes on a buffer whose tiles have landed while those of
 // kt + 1 are on their way to the other.  The two buffers are LDS variables of their own and appear by
 // name in code of their own, so that the compiler does not make the reads of one wait for the other.
@@ -366,6 +459,60 @@ __device__ __forceinline__ void at_walk(int n, char* even, char* odd, const F& f
   }
 }
 
+// Products of a part that crosses the diagonal give masked rows the weight 0, and 0 times an infinity or a NaN
+// is a NaN, which belongs to no row that does not see them.  So where a wave's results are not finite, it looks
+// at the 32 rows x of its diagonal part: a result that only rows hidden from it can have spoilt is computed
+// again from the tensors, adding up only what its row sees.  Lane l has own row l % 32 and dims l / 32 HD / 2 ..
+// of it here.  (After the stores, so that nothing of it is in the loops.)
+template <int N>
+__device__ __forceinline__ bool at_spoilt(const at_f32x16 (&acc)[N]) {
+  float s = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < N; dt++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) s = fmaf(acc[dt][r], 0.f, s);
+  return __builtin_amdgcn_ballot_w64(s != s) != 0;
+}
+// Whether some dim of the lane's is not finite in a hidden row of x (n rows, stride apart) and finite in all
+// that its own row i sees: rows 0 .. i, or (UP) i .. n - 1.
+template <typename O, bool UP>
+__device__ __forceinline__ bool at_hidden(const O* x, size_t stride, int n, int i, int d0, int dims, int hd) {
+  bool need = false;
+#pragma unroll 1
+  for (int d = d0; d < d0 + dims && d < hd; d++) {
+    bool hidden = false, seen = false;
+#pragma unroll 1
+    for (int r = 0; r < n; r++) {
+      const float v = (float)x[r * stride + d];
+      const bool bad = !(fabsf(v) < INFINITY), sees = UP ? r >= i : r <= i;
+      hidden = hidden || (bad && !sees);
+      seen = seen || (bad && sees);
+    }
+    need = need || (hidden && !seen);
+  }
+  return __builtin_amdgcn_ballot_w64(need) != 0;
+}
+template <typename O>
+__device__ __forceinline__ float at_dot(const O* x, const O* y, int hd) {
+  float s = 0.f;
+#pragma unroll 8
+  for (int d = 0; d < hd; d++) s = fmaf((float)x[d], (float)y[d], s);
+  return s;
+}
+// acc += w * row[d] over the lane's dims
+template <typename O, int N>
+__device__ __forceinline__ void at_add_row(float (&acc)[N], float w, const O* row, int d0, int hd) {
+#pragma unroll
+  for (int d = 0; d < N; d++)
+    if (d0 + d < hd) acc[d] = fmaf(w, (float)row[d0 + d], acc[d]);
+}
+template <typename O, int N>
+__device__ __forceinline__ void at_put_row(O* row, const float (&acc)[N], float f, int d0, int hd) {
+#pragma unroll
+  for (int d = 0; d < N; d++)
+    if (d0 + d < hd) row[d0 + d] = (O)(acc[d] * f);
+}
+
 // Block -> (block of the axis, group = sequence * heads + head) of a causal launch over nblk * G
 // blocks; block 0 of the axis is the one with the most work, and is started first.  Workgroups reach
 // the 8 XCDs round-robin.  Sequences of one length: when 8 divides G, an XCD takes whole neighbouring
@@ -385,6 +532,16 @@ __device__ __forceinline__ AtBlock at_block(int L, int G, int ragged) {
   }
   const int blk = L / G, i = L % G;
   return {blk, ragged && G % 2 == 0 ? (i + blk) % G : i};
+}
+
+// q's columns of a matrix that a kernel reads (its k and v follow), and do's.
+template <typename K>
+__device__ __forceinline__ AtSource<K> at_qkv(const AttnTrain& a) {
+  return {static_cast<const typename K::E*>(a.in), a.in_part, a.in_cols, a.in_hd};
+}
+template <typename K>
+__device__ __forceinline__ AtSource<K> at_do(const AttnTrain& a) {
+  return {static_cast<const typename K::E*>(a.in_do), a.do_part, a.do_cols, a.in_hd};
 }
 
 __device__ __forceinline__ int at_len(const AttnTrain& a, int b) {

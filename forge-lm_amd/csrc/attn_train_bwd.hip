@@ -13,14 +13,17 @@
 
 namespace fh {
 
+hipError_t attn_train_inputs(hipStream_t st, AttnTrain& a, bool bf16, bool backward, size_t scratch_bytes, int cus, bool* split,
+                             bool* vec);
+
 namespace {
 
 // The sum over the four waves of acc^T (dims x the 32 own rows), times f, to rows row0 .. of dst;
 // rows at or past len are zeros, rows at or past T are not written.  os: kJoinFloats<HD>.
 template <int HD>
 constexpr int kJoinFloats = 4 * 32 * ((HD < 64 ? HD : 64) + 1);  // 64 dims at a time
-template <typename E, int HD>
-__device__ __forceinline__ void join_store(float* os, const at_f32x16 (&acc)[HD / 32], float f, E* dst, int row0, int len,
+template <typename O, int HD>
+__device__ __forceinline__ void join_store(float* os, const at_f32x16 (&acc)[HD / 32], float f, O* dst, int row0, int len,
                                            int T, int stride, int hd, int w, int lane, int tid) {
   constexpr int N = HD < 64 ? HD : 64;
 #pragma unroll
@@ -39,7 +42,7 @@ __device__ __forceinline__ void join_store(float* os, const at_f32x16 (&acc)[HD 
       float v = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; k++) v += os[(k * 32 + i) * (N + 1) + d];
-      dst[(size_t)(row0 + i) * stride + d0 + d] = (E)(row0 + i < len ? v * f : 0.f);
+      dst[(size_t)(row0 + i) * stride + d0 + d] = (O)(row0 + i < len ? v * f : 0.f);
     }
   }
 }
@@ -52,11 +55,75 @@ __device__ __forceinline__ float* stat_part(const AttnTrain& a, size_t head, int
   return a.stats + (head * ((a.T + 31) / 32) + row / 32) * 64;
 }
 
-template <typename E, int HD, int KS, bool VEC>
-__global__ __launch_bounds__(256, sizeof(E) == 4 && HD == 128 ? 1 : 2) void k_attn_backward_q(const AttnTrain a) {
-  typedef AtMma<E, HD> M;
-  typedef AtPlan<E, HD, KS, VEC> P;
-  constexpr bool kAhead = sizeof(E) == 2 && HD <= 64;  // registers for the transposed operand before the exponentials
+// p and ds of query i and key j, as the kernels have them
+template <typename O>
+__device__ __forceinline__ void score_again(const AttnTrain& a, int b, int h, int i, int j, float& p, float& ds) {
+  const O* x = static_cast<const O*>(a.qkv) + (size_t)b * a.T * a.qkv_cols;
+  const O* k = x + (size_t)j * a.qkv_cols + (size_t)(a.H + h / (a.H / a.Hk)) * a.hd;
+  const size_t orow = ((size_t)b * a.T + i) * a.out_cols + (size_t)h * a.hd, head = (size_t)b * a.H + h;
+  const O* dout = static_cast<const O*>(a.dout) + orow;
+  const float D = at_dot(dout, static_cast<const O*>(a.out) + orow, a.hd);
+  p = __builtin_amdgcn_exp2f(
+      fmaf(at_dot(x + (size_t)i * a.qkv_cols + (size_t)h * a.hd, k, a.hd), a.scale * kLog2e, -a.lse[head * a.T + i] * kLog2e));
+  ds = p * (at_dot(dout, k + (size_t)a.Hk * a.hd, a.hd) - D);
+}
+// at_spoilt: dq of the rows from t0 on.
+template <typename O, int HD>
+__device__ __forceinline__ void backward_q_again(const AttnTrain& a, int b, int h, int t0, int len, int lane) {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // the stores before
+  const O* k = static_cast<const O*>(a.qkv) + (size_t)b * a.T * a.qkv_cols + (size_t)(a.H + h / (a.H / a.Hk)) * a.hd;
+  const int q = t0 + (lane & 31), d0 = (lane >> 5) * (HD / 2);
+  if (t0 >= len || !at_hidden<O, false>(k + (size_t)t0 * a.qkv_cols, a.qkv_cols, min(32, len - t0), lane & 31, d0, HD / 2, a.hd))
+    return;
+  if (q >= len) return;
+  float acc[HD / 2] = {};
+#pragma unroll 1
+  for (int j = 0; j <= q; j++) {
+    float p, ds;
+    score_again<O>(a, b, h, q, j, p, ds);
+    at_add_row(acc, ds, k + (size_t)j * a.qkv_cols, d0, a.hd);
+  }
+  at_put_row(static_cast<O*>(a.dqkv) + ((size_t)b * a.T + q) * a.qkv_cols + (size_t)h * a.hd, acc, a.scale, d0, a.hd);
+}
+// at_spoilt: dk and dv of the rows from k0 on.
+template <typename O, int HD>
+__device__ __forceinline__ void backward_kv_again(const AttnTrain& a, int b, int kvh, int k0, int len, int lane) {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // the stores before
+  const int group = a.H / a.Hk, key = k0 + (lane & 31), d0 = (lane >> 5) * (HD / 2);
+  const size_t row0 = (size_t)b * a.T;
+  auto from = [&](int which, int h, int i) {  // a row of q or do
+    return which ? static_cast<const O*>(a.dout) + (row0 + i) * a.out_cols + (size_t)h * a.hd
+                 : static_cast<const O*>(a.qkv) + (row0 + i) * a.qkv_cols + (size_t)h * a.hd;
+  };
+#pragma unroll 1
+  for (int which = 0; which < 2; which++) {  // dk, dv
+    bool need = false;
+#pragma unroll 1
+    for (int h = kvh * group; h < (kvh + 1) * group && k0 < len; h++)
+      need = need || at_hidden<O, true>(from(which, h, k0), which ? a.out_cols : a.qkv_cols, min(32, len - k0), lane & 31, d0,
+                                        HD / 2, a.hd);
+    if (!need || key >= len) continue;
+    float acc[HD / 2] = {};
+#pragma unroll 1
+    for (int h = kvh * group; h < (kvh + 1) * group; h++)
+#pragma unroll 1
+      for (int i = key; i < len; i++) {
+        float p, ds;
+        score_again<O>(a, b, h, i, key, p, ds);
+        at_add_row(acc, which ? p : ds, from(which, h, i), d0, a.hd);
+      }
+    O* to = static_cast<O*>(a.dqkv) + (row0 + key) * a.qkv_cols + (size_t)(a.H + kvh + (which ? a.Hk : 0)) * a.hd;
+    at_put_row(to, acc, which ? 1.f : a.scale, d0, a.hd);
+  }
+}
+
+template <typename K, int HD, int KS, bool VEC>
+__global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O) == 4 ? 1 : 2) void k_attn_backward_q(
+    const AttnTrain a) {
+  typedef AtMma<K, HD> M;
+  typedef typename K::E E;
+  typedef typename K::O O;
+  typedef AtPlan<K, HD, KS, VEC> P;
   constexpr int kJoin = KS == 4 ? kJoinFloats<HD> * 4 : 0, kHalf = P::kBytes / 2;
   // KS == 1: [K, V] tiles, and the same for odd steps; KS == 4: the waves' K tiles, and their V tiles
   constexpr int kFirst = KS == 1 ? P::kBytes : kHalf > kJoin ? kHalf : kJoin;
@@ -69,9 +136,8 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && HD == 128 ? 1 : 2) void k_at
   const int t0 = (nqb - 1 - at.blk) * P::kOwn, len = at_len(a, b);
   const int qw0 = t0 + (KS == 1 ? 32 * w : 0), q = qw0 + (lane & 31);
   const size_t row0 = (size_t)b * a.T;
-  const E* seq = static_cast<const E*>(a.qkv) + row0 * a.qkv_cols;
-  const E* kb = seq + (size_t)(a.H + kvh) * a.hd;
-  const E* vb = kb + (size_t)a.Hk * a.hd;
+  const AtSource<K> x = at_qkv<K>(a), xo = at_do<K>(a);
+  const int qc = h * a.in_hd, kc = (a.H + kvh) * a.in_hd, vc = kc + a.Hk * a.in_hd;  // columns
   const float sl2 = a.scale * kLog2e;
 
   at_f32x16 dq[HD / 32];
@@ -80,32 +146,37 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && HD == 128 ? 1 : 2) void k_at
 
   if (t0 < len) {
     const int n = min(32, len - qw0);
-    const typename M::Own own = M::template own<VEC>(
-        at_rows(seq + (size_t)qw0 * a.qkv_cols + (size_t)h * a.hd, n, a.qkv_cols, a.hd), lane & 31, lane);
-    const size_t orow = (row0 + qw0) * a.out_cols + (size_t)h * a.hd;
-    const typename M::Own dout =
-        M::template own<VEC>(at_rows(static_cast<const E*>(a.dout) + orow, n, a.out_cols, a.hd), lane & 31, lane);
-    float D = M::dot(dout, M::template own<VEC>(at_rows(static_cast<const E*>(a.out) + orow, n, a.out_cols, a.hd),
-                                                lane & 31, lane));
-    D += __shfl_xor(D, 32, 64);
-    const float lse2 = q < len ? a.lse[(size_t)at.g * a.T + q] * kLog2e : INFINITY;
-    if ((KS == 1 || w == 0) && qw0 < len)
-      stat_part(a, at.g, qw0)[lane] = lane >= 32 ? -D : sizeof(E) == 4 ? -lse2 : -lse2 / sl2;
-    auto rows_of = [&](const E* base, int k0) {
-      return at_rows(base + (size_t)k0 * a.qkv_cols, min(P::kRows, len - k0), a.qkv_cols, a.hd);
+    typename M::Own own, dout;
+    at_own<K, HD, VEC>(own, x, row0 + qw0, qc, n, lane);
+    at_own<K, HD, VEC>(dout, xo, row0 + qw0, qc, n, lane);
+    float D, lse2;
+    if constexpr (K::kParts > 1) {  // the statistics came with the parts
+      const float* st = stat_part(a, at.g, qw0) + (lane & 31);
+      lse2 = q < len ? -st[0] : INFINITY;
+      D = q < len ? -st[32] : 0.f;
+    } else {
+      typename M::Own o;
+      at_own<K, HD, VEC>(o, AtSource<K>{static_cast<const E*>(a.out), 0, a.out_cols, a.hd}, row0 + qw0, qc, n, lane);
+      D = M::dot(dout.v[0], o.v[0]);
+      D += __shfl_xor(D, 32, 64);
+      lse2 = q < len ? a.lse[(size_t)at.g * a.T + q] * kLog2e : INFINITY;
+      if ((KS == 1 || w == 0) && qw0 < len)
+        stat_part(a, at.g, qw0)[lane] = lane >= 32 ? -D : sizeof(O) == 4 ? -lse2 : -lse2 / sl2;
+    }
+    auto load = [&](E* tile, int col, int k0, int wave) {
+      at_load<K, HD, KS, VEC>(tile, x, row0 + k0, col, len - k0, wave, lane);
     };
     // the 32 keys from k0 on, tile rows r0 ..; the calls come where the V tile has been read for the last
     // time, and before the K tile is read
     auto part = [&](int k0, const E* Ks, const E* Vs, int r0, auto&& v_read, auto&& k_wait) {
       at_f32x16 s, dp;
-      typename M::Cols kc;
       at_zero(dp);
-      M::rows(dp, M::load_rows(Vs, r0, lane), dout);
+      M::rows(dp, Vs, P::kSub, r0, dout, lane);
       v_read();
       k_wait();
       at_zero(s);
-      M::rows(s, M::load_rows(Ks, r0, lane), own);
-      if (kAhead) kc = M::load_cols(Ks, r0, lane);
+      M::rows(s, Ks, P::kSub, r0, own, lane);
+      const typename M::Cols kf = M::load_cols(Ks, P::kSub, r0, lane);
 #pragma unroll
       for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl2, -lse2)) * (dp[r] - D);
       if (k0 + 31 > qw0) {                          // the part crosses the diagonal
@@ -114,14 +185,13 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && HD == 128 ? 1 : 2) void k_at
         for (int r = 0; r < 16; r++)
           if (at_row0(r) > left) s[r] = 0.f;
       }
-      if (!kAhead) kc = M::load_cols(Ks, r0, lane);
-      M::cols(dq, kc, s, lane);
+      M::cols(dq, kf, s, lane);
     };
     if constexpr (KS == 1) {
       auto fetch = [&](int kt, char* buf) {
         E* t = reinterpret_cast<E*>(buf);
-        at_load<E, HD, KS, VEC>(t, rows_of(kb, kt * P::kRows), w, lane);
-        at_load<E, HD, KS, VEC>(t + P::kTile, rows_of(vb, kt * P::kRows), w, lane);
+        load(t, kc, kt * P::kRows, w);
+        load(t + P::kTile, vc, kt * P::kRows, w);
       };
       auto compute = [&](int kt, const char* buf) {
         const E* t = reinterpret_cast<const E*>(buf);
@@ -137,38 +207,41 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 && HD == 128 ? 1 : 2) void k_at
       E *Ks = reinterpret_cast<E*>(smem) + w * P::kTile, *Vs = reinterpret_cast<E*>(odd) + w * P::kTile;
       const int last = t0 / 32;
       if (w <= last) {
-        at_load<E, HD, KS, VEC>(Vs, rows_of(vb, 32 * w), 0, lane);
-        at_load<E, HD, KS, VEC>(Ks, rows_of(kb, 32 * w), 0, lane);
+        load(Vs, vc, 32 * w, 0);
+        load(Ks, kc, 32 * w, 0);
       }
       for (int p = w; p <= last; p += 4) {  // (past the last part nothing is in reach, and zeros arrive)
         at_wait<P::kLoads>();
         part(32 * p, Ks, Vs, 0,
              [&] {
                at_wait<-1>();
-               at_load<E, HD, KS, VEC>(Vs, rows_of(vb, 32 * (p + 4)), 0, lane);
+               load(Vs, vc, 32 * (p + 4), 0);
              },
              [&] { at_wait<P::kLoads>(); });
         at_wait<-1>();
-        at_load<E, HD, KS, VEC>(Ks, rows_of(kb, 32 * (p + 4)), 0, lane);
+        load(Ks, kc, 32 * (p + 4), 0);
       }
     }
   }
-  E* dst = static_cast<E*>(a.dqkv) + row0 * a.qkv_cols + (size_t)h * a.hd;
+  O* dst = static_cast<O*>(a.dqkv) + row0 * a.qkv_cols + (size_t)h * a.hd;
   if constexpr (KS == 1) {
     at_landed();  // the tiles' LDS is free
     if (qw0 >= a.T) return;
-    at_store<E, HD, VEC, P::kStaged>(dst + (size_t)qw0 * a.qkv_cols, a.qkv_cols, dq, a.scale, a.T - qw0, len - qw0, a.hd,
-                         reinterpret_cast<E*>(smem) + w * 32 * HD, lane);
+    at_store<O, HD, VEC, P::kOut>(dst + (size_t)qw0 * a.qkv_cols, a.qkv_cols, dq, a.scale, a.T - qw0, len - qw0, a.hd,
+                                   reinterpret_cast<O*>(smem) + w * P::kOut * HD, lane);
+    if (at_spoilt(dq)) backward_q_again<O, HD>(a, b, h, qw0, len, lane);
   } else {
-    join_store<E, HD>(reinterpret_cast<float*>(smem), dq, a.scale, dst, t0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
+    join_store<O, HD>(reinterpret_cast<float*>(smem), dq, a.scale, dst, t0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
+    if (__syncthreads_or(at_spoilt(dq)) && w == 0) backward_q_again<O, HD>(a, b, h, t0, len, lane);
   }
 }
 
-template <typename E, int HD, int KS, bool VEC>
-__global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(const AttnTrain a) {
-  typedef AtMma<E, HD> M;
-  typedef AtPlan<E, HD, KS, VEC> P;
-  constexpr bool kAhead = sizeof(E) == 2 && HD <= 64;  // registers for the transposed operand before the exponentials
+template <typename K, int HD, int KS, bool VEC>
+__global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_kv(const AttnTrain a) {
+  typedef AtMma<K, HD> M;
+  typedef typename K::E E;
+  typedef typename K::O O;
+  typedef AtPlan<K, HD, KS, VEC> P;
   constexpr int kJoin = KS == 4 ? kJoinFloats<HD> * 4 : 0, kHalf = P::kBytes / 2;
   // KS == 1: [Q, dO] tiles, and the same for odd steps; KS == 4: the waves' Q tiles, and their dO tiles
   constexpr int kFirst = KS == 1 ? P::kBytes : kHalf > kJoin ? kHalf : kJoin;
@@ -182,7 +255,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
   const int k0 = at.blk * P::kOwn, len = at_len(a, b);
   const int kw0 = k0 + (KS == 1 ? 32 * w : 0), key = kw0 + (lane & 31);
   const size_t row0 = (size_t)b * a.T;
-  const E* seq = static_cast<const E*>(a.qkv) + row0 * a.qkv_cols;
+  const AtSource<K> x = at_qkv<K>(a), xo = at_do<K>(a);
   const float sl2 = a.scale * kLog2e;
 
   at_f32x16 dk[HD / 32], dv[HD / 32];
@@ -192,18 +265,13 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
     at_zero(dv[dt]);
   }
   if (k0 < len) {
-    const int n = min(32, len - kw0);
-    const E* kb = seq + (size_t)kw0 * a.qkv_cols + (size_t)(a.H + kvh) * a.hd;
-    const typename M::Own ko = M::template own<VEC>(at_rows(kb, n, a.qkv_cols, a.hd), lane & 31, lane);
-    const typename M::Own vo =
-        M::template own<VEC>(at_rows(kb + (size_t)a.Hk * a.hd, n, a.qkv_cols, a.hd), lane & 31, lane);
+    const int n = min(32, len - kw0), kc = (a.H + kvh) * a.in_hd;
+    typename M::Own ko, vo;
+    at_own<K, HD, VEC>(ko, x, row0 + kw0, kc, n, lane);
+    at_own<K, HD, VEC>(vo, x, row0 + kw0, kc + a.Hk * a.in_hd, n, lane);
     const int head0 = kvh * group;
-    auto q_rows = [&](int g, int q0) {
-      return at_rows(seq + (size_t)q0 * a.qkv_cols + (size_t)(head0 + g) * a.hd, min(P::kRows, len - q0), a.qkv_cols, a.hd);
-    };
-    auto do_rows = [&](int g, int q0) {
-      return at_rows(static_cast<const E*>(a.dout) + (row0 + q0) * a.out_cols + (size_t)(head0 + g) * a.hd,
-                     min(P::kRows, len - q0), a.out_cols, a.hd);
+    auto load = [&](E* tile, const AtSource<K>& m, int g, int q0, int wave) {
+      at_load<K, HD, KS, VEC>(tile, m, row0 + q0, (size_t)(head0 + g) * a.in_hd, len - q0, wave, lane);
     };
     // a part's statistics into LDS (past the length: zeros, which no part that counts reads)
     auto load_stat = [&](float* to, int g, int q0) {
@@ -220,13 +288,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
     auto part = [&](int r0, const E* Qs, const E* Os, int i0, const float* sp, auto&& q_wait, auto&& do_read) {
       at_f32x16 s, dp;
       const float* st = sp + 4 * (lane >> 5);
-      typename M::Cols oc;
-      if constexpr (sizeof(E) == 4) {
+      if constexpr (sizeof(O) == 4) {
         at_zero(dp);
         at_zero(s);
-        M::rows(dp, M::load_rows(Os, i0, lane), vo);
+        M::rows(dp, Os, P::kSub, i0, vo, lane);
         q_wait();
-        M::rows(s, M::load_rows(Qs, i0, lane), ko);
       } else {
         q_wait();
 #pragma unroll
@@ -235,14 +301,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
           s[4 * c] = l.x, s[4 * c + 1] = l.y, s[4 * c + 2] = l.z, s[4 * c + 3] = l.w;
           dp[4 * c] = d.x, dp[4 * c + 1] = d.y, dp[4 * c + 2] = d.z, dp[4 * c + 3] = d.w;
         }
-        M::rows(dp, M::load_rows(Os, i0, lane), vo);
-        M::rows(s, M::load_rows(Qs, i0, lane), ko);
-        if (kAhead) oc = M::load_cols(Os, i0, lane);
+        M::rows(dp, Os, P::kSub, i0, vo, lane);
       }
+      M::rows(s, Qs, P::kSub, i0, ko, lane);
+      const typename M::Cols of = M::load_cols(Os, P::kSub, i0, lane);
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         float l4[4], d4[4];
-        if constexpr (sizeof(E) == 4) {
+        if constexpr (sizeof(O) == 4) {
           const float4 l = *reinterpret_cast<const float4*>(st + 8 * c), d = *reinterpret_cast<const float4*>(st + 32 + 8 * c);
           l4[0] = l.x, l4[1] = l.y, l4[2] = l.z, l4[3] = l.w;
           d4[0] = d.x, d4[1] = d.y, d4[2] = d.z, d4[3] = d.w;
@@ -250,7 +316,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int r = 4 * c + e;
-          if constexpr (sizeof(E) == 4) {
+          if constexpr (sizeof(O) == 4) {
             s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl2, l4[e]));
             dp[r] = s[r] * (dp[r] + d4[e]);
           } else {
@@ -265,18 +331,17 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
         for (int r = 0; r < 16; r++)
           if (at_row0(r) < first) s[r] = dp[r] = 0.f;
       }
-      if (!kAhead) oc = M::load_cols(Os, i0, lane);
-      M::cols(dv, oc, s, lane);
+      M::cols(dv, of, s, lane);
       do_read();
-      M::cols(dk, M::load_cols(Qs, i0, lane), dp, lane);
+      M::cols(dk, M::load_cols(Qs, P::kSub, i0, lane), dp, lane);
     };
     const int tiles = (len - k0 + P::kRows - 1) / P::kRows;  // of a head
     if constexpr (KS == 1) {
       int fg = 0, fq = k0, q0 = k0;  // head and first row of the tile to be requested next; first row of this one
       auto fetch = [&](int, char* buf) {
         E* t = reinterpret_cast<E*>(buf);
-        at_load<E, HD, KS, VEC>(t, q_rows(fg, fq), w, lane);
-        at_load<E, HD, KS, VEC>(t + P::kTile, do_rows(fg, fq), w, lane);
+        load(t, x, fg, fq, w);
+        load(t + P::kTile, xo, fg, fq, w);
         if (w < P::kParts) load_stat(buf == smem ? stat[w] : stat_odd[w], fg, fq + 32 * w);
         fq += P::kRows;
         if (fq >= len) {
@@ -302,8 +367,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
       int g = 0, p = w;  // this wave's part: of all heads' parts every fourth
       while (p >= tiles && g < group) p -= tiles, g++;
       if (g < group) {
-        at_load<E, HD, KS, VEC>(Os, do_rows(g, k0 + 32 * p), 0, lane);
-        at_load<E, HD, KS, VEC>(Qs, q_rows(g, k0 + 32 * p), 0, lane);
+        load(Os, xo, g, k0 + 32 * p, 0);
+        load(Qs, x, g, k0 + 32 * p, 0);
         load_stat(stat[w], g, k0 + 32 * p);
       }
       while (g < group) {
@@ -315,67 +380,75 @@ __global__ __launch_bounds__(256, HD == 128 ? 1 : 2) void k_attn_backward_kv(con
         part(r0, Qs, Os, 0, stat[w], [] { at_wait<0>(); },
              [&] {
                at_wait<-1>();
-               at_load<E, HD, KS, VEC>(Os, do_rows(ng, nq), 0, lane);
+               load(Os, xo, ng, nq, 0);
              });
         at_wait<-1>();
-        at_load<E, HD, KS, VEC>(Qs, q_rows(ng, nq), 0, lane);
+        load(Qs, x, ng, nq, 0);
         load_stat(stat[w], ng, nq);
       }
     }
   }
-  E* dst = static_cast<E*>(a.dqkv) + row0 * a.qkv_cols + (size_t)(a.H + kvh) * a.hd;
-  E* dstv = dst + (size_t)a.Hk * a.hd;
+  O* dst = static_cast<O*>(a.dqkv) + row0 * a.qkv_cols + (size_t)(a.H + kvh) * a.hd;
+  O* dstv = dst + (size_t)a.Hk * a.hd;
   if constexpr (KS == 1) {
     at_landed();  // the tiles' LDS is free
     if (kw0 >= a.T) return;
-    E* tile = reinterpret_cast<E*>(smem) + w * 32 * HD;
-    at_store<E, HD, VEC, P::kStaged>(dst + (size_t)kw0 * a.qkv_cols, a.qkv_cols, dk, a.scale, a.T - kw0, len - kw0, a.hd, tile, lane);
-    at_store<E, HD, VEC, P::kStaged>(dstv + (size_t)kw0 * a.qkv_cols, a.qkv_cols, dv, 1.f, a.T - kw0, len - kw0, a.hd, tile, lane);
+    O* tile = reinterpret_cast<O*>(smem) + w * P::kOut * HD;
+    at_store<O, HD, VEC, P::kOut>(dst + (size_t)kw0 * a.qkv_cols, a.qkv_cols, dk, a.scale, a.T - kw0, len - kw0, a.hd, tile, lane);
+    at_store<O, HD, VEC, P::kOut>(dstv + (size_t)kw0 * a.qkv_cols, a.qkv_cols, dv, 1.f, a.T - kw0, len - kw0, a.hd, tile, lane);
+    if (at_spoilt(dk) || at_spoilt(dv)) backward_kv_again<O, HD>(a, b, kvh, kw0, len, lane);
   } else {
     float* os = reinterpret_cast<float*>(smem);
-    join_store<E, HD>(os, dk, a.scale, dst, k0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
-    join_store<E, HD>(os, dv, 1.f, dstv, k0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
+    join_store<O, HD>(os, dk, a.scale, dst, k0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
+    join_store<O, HD>(os, dv, 1.f, dstv, k0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
+    if (__syncthreads_or(at_spoilt(dk) || at_spoilt(dv)) && w == 0) backward_kv_again<O, HD>(a, b, kvh, k0, len, lane);
   }
 }
 
-template <typename E, int HD>
-void backward_hd(hipStream_t st, const AttnTrain& a, bool vec, int cus) {
+template <typename K, int HD, bool VEC>
+void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   const size_t wide = (size_t)((a.T + 127) / 128), narrow = (size_t)((a.T + 31) / 32);
   const size_t gq = (size_t)a.B * a.H, gk = (size_t)a.B * a.Hk;
-  if (!vec) {
-    hipLaunchKernelGGL((k_attn_backward_q<E, HD, 1, false>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((k_attn_backward_kv<E, HD, 1, false>), dim3((unsigned)(wide * gk)), dim3(256), 0, st, a);
-    return;
+  bool few_q = at_few<K, HD>(wide * gq, cus), few_k = at_few<K, HD>(wide * gk, cus);
+  if constexpr (VEC) {
+    if (few_q)
+      hipLaunchKernelGGL((k_attn_backward_q<K, HD, 4, VEC>), dim3((unsigned)(narrow * gq)), dim3(256), 0, st, a);
+  } else {
+    few_q = few_k = false;
   }
-  if (wide * gq < (size_t)cus)
-    hipLaunchKernelGGL((k_attn_backward_q<E, HD, 4, true>), dim3((unsigned)(narrow * gq)), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_attn_backward_q<E, HD, 1, true>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
-  if (wide * gk < (size_t)cus)
-    hipLaunchKernelGGL((k_attn_backward_kv<E, HD, 4, true>), dim3((unsigned)(narrow * gk)), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_attn_backward_kv<E, HD, 1, true>), dim3((unsigned)(wide * gk)), dim3(256), 0, st, a);
+  if (!few_q) hipLaunchKernelGGL((k_attn_backward_q<K, HD, 1, VEC>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
+  if constexpr (VEC) {
+    if (few_k)
+      hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 4, VEC>), dim3((unsigned)(narrow * gk)), dim3(256), 0, st, a);
+  }
+  if (!few_k) hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 1, VEC>), dim3((unsigned)(wide * gk)), dim3(256), 0, st, a);
 }
 
-template <typename E>
-void backward(hipStream_t st, const AttnTrain& a, bool vec, int cus) {
+template <typename K, bool VEC>
+void backward(hipStream_t st, const AttnTrain& a, int cus) {
   if (a.hd <= 32)
-    backward_hd<E, 32>(st, a, vec, cus);
+    backward_hd<K, 32, VEC>(st, a, cus);
   else if (a.hd <= 64)
-    backward_hd<E, 64>(st, a, vec, cus);
-  else
-    backward_hd<E, 128>(st, a, vec, cus);
+    backward_hd<K, 64, VEC>(st, a, cus);
+  else if constexpr (K::kParts == 1)
+    backward_hd<K, 128, VEC>(st, a, cus);
 }
 
 }  // namespace
 
-hipError_t launch_attn_backward(hipStream_t st, const AttnTrain& a, bool bf16, int cus) {
-  if (!attn_train_fits(a) || !a.qkv || !a.out || !a.lse || !a.dout || !a.dqkv || !a.stats) return hipErrorInvalidValue;
-  const bool vec = attn_train_vec(a, bf16 ? 2 : 4);
-  if (bf16)
-    backward<__bf16>(st, a, vec, cus);
+hipError_t launch_attn_backward(hipStream_t st, AttnTrain a, bool bf16, size_t scratch_bytes, int cus) {
+  if (!attn_train_fits(a) || !a.qkv || !a.out || !a.lse || !a.dout || !a.dqkv || !a.scratch ||
+      scratch_bytes < attn_train_scratch(a, bf16, true, false, cus))
+    return hipErrorInvalidValue;
+  bool split, vec;
+  const hipError_t e = attn_train_inputs(st, a, bf16, true, scratch_bytes, cus, &split, &vec);
+  if (e != hipSuccess) return e;
+  if (split)
+    backward<AtSplit, true>(st, a, cus);
+  else if (bf16)
+    vec ? backward<AtBf16, true>(st, a, cus) : backward<AtBf16, false>(st, a, cus);
   else
-    backward<float>(st, a, vec, cus);
+    vec ? backward<AtF32, true>(st, a, cus) : backward<AtF32, false>(st, a, cus);
   return hipGetLastError();
 }
 

@@ -244,23 +244,25 @@ struct AttnTrain {
   float* lse;        // [B][H][T], as out
   const void* dout;  // backward
   void* dqkv;
-  float* stats;  // backward's scratch, attn_train_stats(a) floats
   int B, T, H, Hk, hd, qkv_cols, out_cols;
   float scale;          // positive
   int ragged;           // lengths in lens_dev, or in lens where that is null (B <= kAttnTrainLens)
   const int* lens_dev;
   int lens[kAttnTrainLens];
+  void* scratch;  // attn_train_scratch bytes (forward: null where that is 0)
+  // filled by the launch: what the kernels read in place of qkv and dout (these, or their parts)
+  const void *in, *in_do;
+  size_t in_part, do_part;
+  int in_cols, do_cols, in_hd;
+  float* stats;  // a row's lse and D, [B][H][32-row part][64]
 };
 bool attn_train_fits(const AttnTrain& a);
-inline size_t attn_train_stats(const AttnTrain& a) { return (size_t)a.B * a.H * ((a.T + 31) / 32) * 64; }
-// whether every row of a head can be moved by 16 bytes (esize: bytes of an element)
-inline bool attn_train_vec(const AttnTrain& a, int esize) {
-  auto ok = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-  const int n = 16 / esize;
-  return a.hd % n == 0 && a.qkv_cols % n == 0 && a.out_cols % n == 0 && ok(a.qkv) && ok(a.out) && ok(a.dout) && ok(a.dqkv);
-}
-hipError_t launch_attn_forward(hipStream_t st, const AttnTrain& a, bool bf16, int cus);
-hipError_t launch_attn_backward(hipStream_t st, const AttnTrain& a, bool bf16, int cus);
+// Bytes of scratch that a launch uses; with `split` false, that it cannot do without (the fp32 values of
+// larger calls are otherwise multiplied as three bf16 parts each).
+size_t attn_train_scratch(const AttnTrain& a, bool bf16, bool backward, bool split, int cus);
+// scratch_bytes: at least the smaller of the two
+hipError_t launch_attn_forward(hipStream_t st, AttnTrain a, bool bf16, size_t scratch_bytes, int cus);
+hipError_t launch_attn_backward(hipStream_t st, AttnTrain a, bool bf16, size_t scratch_bytes, int cus);
 
 // Distillation from a teacher's top logits (distill.hip): row losses, and gradients where dlogits is
 // not null (it may be logits); then their sum in double into *sum (or added to it).  targets and sum may be

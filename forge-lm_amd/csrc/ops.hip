@@ -1738,6 +1738,28 @@ int attention_args(const void* qkv, int qkv_cols, const void* out, int out_cols,
   return FH_OK;
 }
 
+// a's scratch and, where they do not travel in the arguments, its lengths on the device (after the scratch)
+int attention_scratch(fh_context* c, OpsState* o, AttnTrain* a, const int32_t* lengths, bool bf16, bool backward,
+                      size_t* bytes) {
+  const int cus = context_cus(c);
+  const bool upload = lengths && a->B > kAttnTrainLens;
+  const size_t ints = upload ? (size_t)a->B * sizeof(int32_t) : 0, least = attn_train_scratch(*a, bf16, backward, false, cus);
+  *bytes = attn_train_scratch(*a, bf16, backward, true, cus);
+  void* p = nullptr;
+  if (*bytes > least && ops_scratch(c, o, *bytes + ints, &p) != FH_OK) p = nullptr;  // a full device: without the parts
+  if (!p) {
+    *bytes = least;
+    if (least + ints) FH_TRY(ops_scratch(c, o, least + ints, &p));
+  }
+  a->scratch = *bytes ? p : nullptr;
+  if (upload) {
+    int* dev = reinterpret_cast<int*>(static_cast<char*>(p) + *bytes);
+    FH_TRY(copy_ints(c, o, lengths, (size_t)a->B, dev));
+    a->lens_dev = dev;
+  }
+  return FH_OK;
+}
+
 bool element_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == FH_DTYPE_BF16 ? 1 : 3)) == 0; }
 
 }  // namespace
@@ -1753,12 +1775,9 @@ int fh_op_attention_forward(fh_context* c, const void* qkv, int qkv_cols, void* 
   OPS_ARG(element_aligned(qkv, dtype) && element_aligned(out, dtype) && aligned4(lse), "buffer not aligned to its elements");
   OPS_ARG(out != qkv && (const void*)lse != qkv && (void*)lse != out, "the outputs must be buffers of their own");
   OPS_PROLOGUE(c);
-  if (lengths && batch > kAttnTrainLens) {
-    int* dev = nullptr;
-    FH_TRY(upload_ints(c, ops_, lengths, (size_t)batch, &dev));
-    a.lens_dev = dev;
-  }
-  HIP_TRY(launch_attn_forward(st_, a, dtype == FH_DTYPE_BF16, context_cus(c)));
+  size_t bytes = 0;
+  FH_TRY(attention_scratch(c, ops_, &a, lengths, dtype == FH_DTYPE_BF16, false, &bytes));
+  HIP_TRY(launch_attn_forward(st_, a, dtype == FH_DTYPE_BF16, bytes, context_cus(c)));
   return FH_OK;
 }
 
@@ -1775,17 +1794,9 @@ int fh_op_attention_backward(fh_context* c, const void* dout, const void* qkv, i
   OPS_ARG(dqkv != qkv && dqkv != out && dqkv != dout && dqkv != (const void*)lse, "dqkv must be a buffer of its own");
   OPS_PROLOGUE(c);
   a.dout = dout, a.dqkv = dqkv;
-  const size_t sums = attn_train_stats(a);
-  const bool upload = lengths && batch > kAttnTrainLens;
-  void* p = nullptr;
-  FH_TRY(ops_scratch(c, ops_, (sums + (upload ? (size_t)batch : 0)) * 4, &p));
-  a.stats = static_cast<float*>(p);
-  if (upload) {
-    int* dev = reinterpret_cast<int*>(a.stats + sums);
-    FH_TRY(copy_ints(c, ops_, lengths, (size_t)batch, dev));
-    a.lens_dev = dev;
-  }
-  HIP_TRY(launch_attn_backward(st_, a, dtype == FH_DTYPE_BF16, context_cus(c)));
+  size_t bytes = 0;
+  FH_TRY(attention_scratch(c, ops_, &a, lengths, dtype == FH_DTYPE_BF16, true, &bytes));
+  HIP_TRY(launch_attn_backward(st_, a, dtype == FH_DTYPE_BF16, bytes, context_cus(c)));
   return FH_OK;
 }
 

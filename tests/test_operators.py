@@ -230,6 +230,85 @@ def test_attention_sharp_and_flat_rows(fhp, be, std, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,H,Hk,hd,lengths", [
+    (6, 520, 9, 3, 64, None), (6, 520, 9, 9, 40, [520, 1, 519, 0, 300, 32]), (4, 260, 24, 24, 32, None),
+    (1, 1030, 2, 1, 64, None), (2, 1100, 3, 3, 20, [1061, 97]),
+])
+def test_attention_fp32_in_three_parts(fhp, be, B, T, H, Hk, hd, lengths):
+    # long enough that fp32 values are multiplied in bf16 parts, with the bounds of the fp32 products: of a
+    # product a b the parts leave out two of mid times lo, 2^-8 2^-16 each, and add up six exact ones for
+    # every 16 dims, fewer roundings than the hd that the bound counts
+    attention_case(fhp, be, B, T, H, Hk, hd, "f32", lengths=lengths, seed=T + hd)
+
+
+@pytest.mark.gpu
+def test_attention_largest_values_in_parts(fhp, be):
+    # values that would round to infinity in bf16: v and dout alone, so that every sum is in range
+    B, T, H, hd = 1, 1030, 1, 32
+    qkv, dout = np.zeros((T, 3 * hd), np.float32), np.zeros((T, hd), np.float32)
+    top = np.finfo(np.float32).max
+    qkv[:, 2 * hd], dout[-1, 1] = top, top
+    qkv[0, hd + 1], qkv[:, 1] = -1e4, 1.0  # no weight on the first key, but for the first query
+    bq, bd = fhp.DeviceBuffer.from_array(be, qkv), fhp.DeviceBuffer.from_array(be, dout)
+    bo, bl, bg = fhp.DeviceBuffer(be, dout.nbytes), fhp.DeviceBuffer(be, 4 * T), fhp.DeviceBuffer(be, qkv.nbytes)
+    be.attention_forward(bq, bo, bl, B, T, H, hd)
+    be.attention_backward(bd, bq, bo, bl, bg, B, T, H, hd)
+    dv = bg.read(np.float32, T * 3 * hd).reshape(T, -1)[:, 2 * hd + 1].astype(np.float64)
+    want = np.where(np.arange(T) == 0, 0.0, float(top) / (T - 1))  # of the last query, which all others' dout leave alone
+    np.testing.assert_allclose(dv, want, rtol=(T + 40) * F32)
+    for b in (bq, bd, bo, bl, bg):
+        b.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("B,T,H,Hk,hd,dtype", [
+    (1, 75, 4, 2, 64, "f32"), (1, 75, 4, 2, 64, "bf16"), (1, 75, 2, 2, 128, "bf16"), (1, 75, 2, 1, 25, "f32"),
+    (16, 133, 16, 8, 64, "bf16"), (16, 133, 16, 16, 32, "f32"), (1, 1030, 2, 2, 32, "f32"), (9, 520, 6, 6, 16, "f32"),
+])
+def test_attention_rows_depend_on_what_they_see_alone(fhp, be, B, T, H, Hk, hd, dtype, which, value):
+    # row 41 of the last sequence is not finite: o and dq of the rows before it, and what a query's q or
+    # dout cannot reach, are as without it
+    W, Wo, at = (H + 2 * Hk) * hd, H * hd, (B - 1) * T + 41
+    r = np.random.default_rng(8)
+    qkv, dout = r.normal(0, 1, (B * T, W)), r.normal(0, 1, (B * T, Wo))
+    _, qv = stored(qkv, dtype)
+    _, dv = stored(dout, dtype)
+    ref = Attention64(qv, dv, np.full(B, T), B, T, H, Hk, hd, float(np.float32(1 / np.sqrt(hd))), dtype)
+    cols = {"q": slice(0, H * hd), "k": slice(H * hd, (H + Hk) * hd), "v": slice((H + Hk) * hd, W)}
+    if which == "dout":
+        dout[at] = value
+    else:
+        qkv[at, cols[which]] = value
+    raw = lambda x: stored(x, dtype)[0] if dtype == "f32" else np.where(  # noqa: E731
+        np.isinf(x), np.where(x > 0, np.uint16(0x7F80), np.uint16(0xFF80)), stored(np.where(np.isinf(x), 0, x), dtype)[0])
+    qb, db = raw(qkv), raw(dout)
+    bq, bd = fhp.DeviceBuffer.from_array(be, qb), fhp.DeviceBuffer.from_array(be, db)
+    bo, bl, bg = fhp.DeviceBuffer(be, db.nbytes), fhp.DeviceBuffer(be, 4 * B * H * T), fhp.DeviceBuffer(be, qb.nbytes)
+    be.attention_forward(bq, bo, bl, B, T, H, hd, n_kv_heads=Hk, dtype=dtype)
+    be.attention_backward(bd, bq, bo, bl, bg, B, T, H, hd, n_kv_heads=Hk, dtype=dtype)
+    out = values(bo.read(db.dtype, B * T * Wo), dtype).reshape(B * T, Wo)
+    lse = bl.read(np.float32, B * H * T).reshape(B, H, T)
+    g = values(bg.read(qb.dtype, B * T * W), dtype).reshape(B * T, W)
+    row = np.arange(B * T)
+    other = row < (B - 1) * T                      # of other sequences
+    before, after = row < at, other | (row > at)
+    o_ok = np.ones(B * T, bool) if which == "dout" else row != at if which == "q" else before
+    dq_ok = row != at if which in ("q", "dout") else before
+    kv_ok = after if which in ("q", "dout") else other
+    check(out[o_ok], ref.out[o_ok], ref.out_err[o_ok], "out")
+    fine = o_ok.reshape(B, 1, T) & np.ones((B, H, T), bool)
+    check(lse[fine], ref.lse[fine], (ref.lse_err + 4 * F32 * np.abs(ref.lse))[fine], "lse")
+    for c, ok, what in ((cols["q"], dq_ok, "dq"), (cols["k"], kv_ok, "dk"), (cols["v"], kv_ok, "dv")):
+        check(g[ok, c], ref.dqkv[ok, c], ref.dqkv_err[ok, c], what)
+    if np.isnan(value):  # and what sees it shows it
+        assert not np.isfinite(out[at] if which != "dout" else g[at, cols["q"]]).any()
+    for b in (bq, bd, bo, bl, bg):
+        b.free()
+
+
+@pytest.mark.gpu
 def test_attention_gradient_by_differences(fhp, be):
     B, T, H, hd = 1, 5, 2, 4
     r = np.random.default_rng(1)
@@ -403,6 +482,13 @@ def test_distill_empty_rows_and_infinite_logits(fhp, be):
         ids[5, 0] = targets[5]
     distill_case(fhp, be, 7, 1500, 6, "f32", 2.0, 0.5, edit=edit)
     distill_case(fhp, be, 7, 200, 6, "bf16", 1.0, 1.0, edit=edit)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2048, 2049, 20000])
+def test_distill_many_rows(fhp, be, T):
+    # few targets go to the device with the call's work, more are copied first
+    distill_case(fhp, be, T, 33, 4, "f32", 2.0, 0.5, seed=T)
 
 
 @pytest.mark.gpu
