@@ -435,11 +435,12 @@ __device__ __forceinline__ void at_load(typename K::E* tile, const AtSource<K>& 
 
 // KS == 1: the steps 0 .. n - 1 of a walk: step kt computes on a buffer whose tiles have landed while those of
 // kt + 1 are on their way to the other.  The two buffers are LDS variables of their own and appear by
-// name in code of their own, so that the compiler does not make the reads of one wait for the other.
-template <typename P, typename F, typename C>
+// name in code of their own, so that the compiler does not make the reads of one wait for the other.  STARTED:
+// the caller has requested step 0 (kBufs 2).
+template <typename P, bool STARTED = false, typename F, typename C>
 __device__ __forceinline__ void at_walk(int n, char* even, char* odd, const F& fetch, const C& compute) {
   if constexpr (P::kBufs == 2) {
-    fetch(0, even);
+    if (!STARTED) fetch(0, even);
     for (int kt = 0; kt < n; kt += 2) {
       at_landed();
       if (kt + 1 < n) fetch(kt + 1, odd);

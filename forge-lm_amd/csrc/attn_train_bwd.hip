@@ -149,23 +149,40 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
     typename M::Own own, dout;
     at_own<K, HD, VEC>(own, x, row0 + qw0, qc, n, lane);
     at_own<K, HD, VEC>(dout, xo, row0 + qw0, qc, n, lane);
+    std::conditional_t<(K::kParts > 1), char, typename M::Own> o;
+    if constexpr (K::kParts == 1)
+      at_own<K, HD, VEC>(o, AtSource<K>{static_cast<const E*>(a.out), 0, a.out_cols, a.hd}, row0 + qw0, qc, n, lane);
+    // the first tiles are on their way while D waits for the rows above
+    auto load = [&](E* tile, int col, int k0, int wave) {
+      at_load<K, HD, KS, VEC>(tile, x, row0 + k0, col, len - k0, wave, lane);
+    };
+    auto fetch = [&](int kt, char* buf) {
+      E* t = reinterpret_cast<E*>(buf);
+      load(t, kc, kt * P::kRows, w);
+      load(t + P::kTile, vc, kt * P::kRows, w);
+    };
+    E *Ks = reinterpret_cast<E*>(smem) + w * P::kTile, *Vs = reinterpret_cast<E*>(odd) + w * P::kTile;  // KS == 4
+    const int last = t0 / 32;
+    if constexpr (KS == 4) {
+      if (w <= last) {
+        load(Vs, vc, 32 * w, 0);
+        load(Ks, kc, 32 * w, 0);
+      }
+    } else if constexpr (P::kBufs == 2) {
+      fetch(0, smem);
+    }
     float D, lse2;
     if constexpr (K::kParts > 1) {  // the statistics came with the parts
       const float* st = stat_part(a, at.g, qw0) + (lane & 31);
       lse2 = q < len ? -st[0] : INFINITY;
       D = q < len ? -st[32] : 0.f;
     } else {
-      typename M::Own o;
-      at_own<K, HD, VEC>(o, AtSource<K>{static_cast<const E*>(a.out), 0, a.out_cols, a.hd}, row0 + qw0, qc, n, lane);
       D = M::dot(dout.v[0], o.v[0]);
       D += __shfl_xor(D, 32, 64);
       lse2 = q < len ? a.lse[(size_t)at.g * a.T + q] * kLog2e : INFINITY;
       if ((KS == 1 || w == 0) && qw0 < len)
         stat_part(a, at.g, qw0)[lane] = lane >= 32 ? -D : sizeof(O) == 4 ? -lse2 : -lse2 / sl2;
     }
-    auto load = [&](E* tile, int col, int k0, int wave) {
-      at_load<K, HD, KS, VEC>(tile, x, row0 + k0, col, len - k0, wave, lane);
-    };
     // the 32 keys from k0 on, tile rows r0 ..; the calls come where the V tile has been read for the last
     // time, and before the K tile is read
     auto part = [&](int k0, const E* Ks, const E* Vs, int r0, auto&& v_read, auto&& k_wait) {
@@ -188,11 +205,6 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
       M::cols(dq, kf, s, lane);
     };
     if constexpr (KS == 1) {
-      auto fetch = [&](int kt, char* buf) {
-        E* t = reinterpret_cast<E*>(buf);
-        load(t, kc, kt * P::kRows, w);
-        load(t + P::kTile, vc, kt * P::kRows, w);
-      };
       auto compute = [&](int kt, const char* buf) {
         const E* t = reinterpret_cast<const E*>(buf);
 #pragma unroll
@@ -202,14 +214,8 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
             part(k0, t, t + P::kTile, 32 * i, [] {}, [] {});
         }
       };
-      at_walk<P>((min(t0 + P::kOwn, len) - 1) / P::kRows + 1, smem, odd, fetch, compute);
+      at_walk<P, P::kBufs == 2>((min(t0 + P::kOwn, len) - 1) / P::kRows + 1, smem, odd, fetch, compute);
     } else {
-      E *Ks = reinterpret_cast<E*>(smem) + w * P::kTile, *Vs = reinterpret_cast<E*>(odd) + w * P::kTile;
-      const int last = t0 / 32;
-      if (w <= last) {
-        load(Vs, vc, 32 * w, 0);
-        load(Ks, kc, 32 * w, 0);
-      }
       for (int p = w; p <= last; p += 4) {  // (past the last part nothing is in reach, and zeros arrive)
         at_wait<P::kLoads>();
         part(32 * p, Ks, Vs, 0,

@@ -295,8 +295,10 @@ __global__ __launch_bounds__(256) void k_distill_any(const DistillArgs a) {
   slot_grads<E, BT>(a, dz, g, sums[2], target, zt, ids, f, zk);
 }
 
-// sum of the row losses in double, in a fixed order: *to += it, or = it
-__global__ __launch_bounds__(1024) void k_distill_sum(const float* __restrict__ row_loss, int T, double* to, int add) {
+// sum of the row losses in double, in a fixed order: *to += it, or = it with the mark behind it (2 us of 16 rows,
+// 4 of 2048; by the last block of the rows' kernel instead, counted in an atomic: no faster)
+__global__ __launch_bounds__(1024) void k_distill_sum(const float* __restrict__ row_loss, int T, double* to, int add,
+                                                      unsigned long long mark) {
   __shared__ double red[16];
   double s = 0;
   for (int t0 = threadIdx.x; t0 < T; t0 += 8 * 1024) {
@@ -312,7 +314,13 @@ __global__ __launch_bounds__(1024) void k_distill_sum(const float* __restrict__ 
   __syncthreads();
   if (threadIdx.x) return;
   for (int i = 1; i < 16; i++) s += red[i];
-  *to = add ? *to + s : s;
+  if (add) {
+    *to += s;
+    return;
+  }
+  __hip_atomic_store(to, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // the sum has arrived
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(to) + 1, mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 template <typename E, bool GRAD>
@@ -342,7 +350,7 @@ void launch(hipStream_t st, const DistillArgs& a) {
 
 }  // namespace
 
-hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* sum, bool add) {
+hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* sum, bool add, unsigned long long mark) {
   if (a.T <= 0 || a.T >= 1 << 24 || a.V <= 0 || a.K <= 0 || a.K > kDistillTop || !a.logits || !a.targets || !a.top_ids ||
       !a.top_logits || !a.row_loss || !sum)
     return hipErrorInvalidValue;
@@ -350,7 +358,7 @@ hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, doubl
     a.dlogits ? launch<bf16_t, true>(st, a) : launch<bf16_t, false>(st, a);
   else
     a.dlogits ? launch<float, true>(st, a) : launch<float, false>(st, a);
-  hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, st, a.row_loss, a.T, sum, add ? 1 : 0);
+  hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, st, a.row_loss, a.T, sum, add ? 1 : 0, mark);
   return hipGetLastError();
 }
 

@@ -278,7 +278,9 @@ struct DistillArgs {
   int T, V, K, ignore;
   float tau, alpha, inv_count;
 };
-hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* sum, bool add);
+// The losses' sum: with add, added to *sum; else into host memory, sum[0], and once it is there `mark` into
+// sum[1].
+hipError_t launch_distill(hipStream_t st, const DistillArgs& a, bool bf16, double* sum, bool add, unsigned long long mark);
 
 struct SampleArgs {
   const float* logits;  // [B][V] raw ForwardLast logits

@@ -24,6 +24,8 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <cstring>
 #include <type_traits>
 #include <vector>
@@ -1032,7 +1034,8 @@ struct OpsState {
   hipEvent_t stage_done[kStages] = {};
   int stage_next = 0;
   double* acc = nullptr;  // device loss accumulator + a result slot
-  double* result = nullptr;  // pinned host memory that a kernel writes a result to
+  double* result = nullptr;  // pinned host memory that a kernel writes a result and its call's mark to
+  unsigned long long result_mark = 0;
   bool accumulating = false;
   long long accumulated_targets = 0;
 };
@@ -1708,7 +1711,7 @@ int fh_op_adamw_step(fh_context* c, void* w, const void* g, void* m, void* v, in
 namespace {
 
 // The checks that attention's forward and backward share, and `a` filled from them.  lens stays
-// on the host here: attention_lens puts it where the kernels read it.
+// on the host here: attention_scratch puts it where the kernels read it.
 int attention_args(const void* qkv, int qkv_cols, const void* out, int out_cols, const float* lse, const int32_t* lengths,
                    int batch, int T, int n_heads, int n_kv_heads, int head_dim, float scale, int dtype, AttnTrain* a) {
   OPS_ARG(qkv && out && lse, "null buffer");
@@ -1758,6 +1761,23 @@ int attention_scratch(fh_context* c, OpsState* o, AttnTrain* a, const int32_t* l
     a->lens_dev = dev;
   }
   return FH_OK;
+}
+
+// Whether the last call's result came within a millisecond, by its mark in host memory: a stream's
+// synchronization returns 5 us later (the loss of 16 x 2256 logits: 16.4 us a call and 21.3).
+bool result_arrived(const OpsState* o) {
+  const auto* mark = reinterpret_cast<const volatile unsigned long long*>(o->result + 1);
+  const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(1);
+  for (;;) {
+    for (int i = 0; i < 64; i++) {
+      if (*mark == o->result_mark) {
+        std::atomic_thread_fence(std::memory_order_acquire);
+        return true;
+      }
+      __builtin_ia32_pause();
+    }
+    if (std::chrono::steady_clock::now() > until) return false;
+  }
 }
 
 bool element_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == FH_DTYPE_BF16 ? 1 : 3)) == 0; }
@@ -1825,8 +1845,9 @@ int fh_op_distill_loss(fh_context* c, const void* logits, const int32_t* targets
   FH_TRY(ops_scratch(c, ops_, (size_t)T * (sizeof(int32_t) + sizeof(float)), &p));
   if (!ops_->result) {
     void* r = nullptr;
-    HIP_TRY(hipHostMalloc(&r, sizeof(double), hipHostMallocDefault));
+    HIP_TRY(hipHostMalloc(&r, 2 * sizeof(double), hipHostMallocDefault));
     ops_->result = static_cast<double*>(r);
+    std::memset(r, 0, 2 * sizeof(double));
   }
   DistillArgs a{};
   a.logits = logits, a.dlogits = dlogits, a.top_ids = top_ids_dev, a.top_logits = top_logits_dev;
@@ -1843,15 +1864,15 @@ int fh_op_distill_loss(fh_context* c, const void* logits, const int32_t* targets
     a.targets = static_cast<const int*>(p);
   }
   const bool later = ops_->accumulating;  // the loss stays on the device until the accumulation ends
-  HIP_TRY(launch_distill(st_, a, dtype == FH_DTYPE_BF16, later ? ops_->acc : ops_->result, later));
+  HIP_TRY(launch_distill(st_, a, dtype == FH_DTYPE_BF16, later ? ops_->acc : ops_->result, later, ++ops_->result_mark));
   if (staged) FH_TRY(area_used(c, ops_));
   *loss = 0.f;
   if (later) {
     ops_->accumulated_targets += count;
     return FH_OK;
   }
-  HIP_TRY(hipStreamSynchronize(st_));
-  if (count) *loss = (float)(*ops_->result / count);
+  if (!result_arrived(ops_)) HIP_TRY(hipStreamSynchronize(st_));
+  if (count) *loss = (float)(*static_cast<volatile double*>(ops_->result) / count);
   return FH_OK;
 }
 
