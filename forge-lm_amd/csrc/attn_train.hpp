@@ -525,9 +525,9 @@ __device__ __forceinline__ void at_put_row(O* row, const float (&acc)[N], float 
 struct AtBlock {
   int blk, g;
 };
-__device__ __forceinline__ AtBlock at_block(int L, int G, int ragged) {
+__device__ __forceinline__ AtBlock at_block(int L, int blocks, int G, int ragged) {
   if (!ragged && G % 8 == 0) {
-    const int gx = G / 8, i = L >> 3, first = i & ~31, n = min(32, (int)(gridDim.x >> 3) - first);
+    const int gx = G / 8, i = L >> 3, first = i & ~31, n = min(32, (blocks >> 3) - first);
     const int s = i & 32 ? first + n - 1 - (i - first) : i;
     return {s / gx, (L & 7) * gx + s % gx};
   }

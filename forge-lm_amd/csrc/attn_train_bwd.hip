@@ -117,21 +117,28 @@ __device__ __forceinline__ void backward_kv_again(const AttnTrain& a, int b, int
   }
 }
 
+// LDS of a block: two buffers that the walk tells apart by name, and for dk and dv the queries' statistics.
+// KS == 1: a step's two tiles, and those of odd steps; KS == 4: the waves' tiles of one operand, and of the other.
 template <typename K, int HD, int KS, bool VEC>
-__global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O) == 4 ? 1 : 2) void k_attn_backward_q(
-    const AttnTrain a) {
+struct BackLds {
+  typedef AtPlan<K, HD, KS, VEC> P;
+  static constexpr int kJoin = KS == 4 ? kJoinFloats<HD> * 4 : 0, kHalf = P::kBytes / 2;
+  static constexpr int kFirst = KS == 1 ? P::kBytes : kHalf > kJoin ? kHalf : kJoin;
+  static constexpr int kOdd = KS == 4 ? kHalf : P::kBufs == 2 ? P::kBytes : 16;
+  static constexpr int kStats = KS == 4 ? 4 : P::kParts, kStatsOdd = KS == 4 ? 1 : P::kParts;  // 32-row parts
+};
+
+// dq of block `block` of `blocks`.  STATS: the statistics are there; else this computes them for the other kernel.
+template <typename K, int HD, int KS, bool VEC, bool STATS>
+__device__ __forceinline__ void backward_q(const AttnTrain& a, int block, int blocks, char* smem, char* odd) {
   typedef AtMma<K, HD> M;
   typedef typename K::E E;
   typedef typename K::O O;
   typedef AtPlan<K, HD, KS, VEC> P;
-  constexpr int kJoin = KS == 4 ? kJoinFloats<HD> * 4 : 0, kHalf = P::kBytes / 2;
-  // KS == 1: [K, V] tiles, and the same for odd steps; KS == 4: the waves' K tiles, and their V tiles
-  constexpr int kFirst = KS == 1 ? P::kBytes : kHalf > kJoin ? kHalf : kJoin;
-  __shared__ __align__(1024) char smem[kFirst], odd[KS == 4 ? kHalf : P::kBufs == 2 ? P::kBytes : 16];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nqb = (a.T + P::kOwn - 1) / P::kOwn;
-  const AtBlock at = at_block(blockIdx.x, a.B * a.H, a.ragged);
+  const AtBlock at = at_block(block, blocks, a.B * a.H, a.ragged);
   const int b = at.g / a.H, h = at.g % a.H, kvh = h / (a.H / a.Hk);
   const int t0 = (nqb - 1 - at.blk) * P::kOwn, len = at_len(a, b);
   const int qw0 = t0 + (KS == 1 ? 32 * w : 0), q = qw0 + (lane & 31);
@@ -149,8 +156,8 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
     typename M::Own own, dout;
     at_own<K, HD, VEC>(own, x, row0 + qw0, qc, n, lane);
     at_own<K, HD, VEC>(dout, xo, row0 + qw0, qc, n, lane);
-    std::conditional_t<(K::kParts > 1), char, typename M::Own> o;
-    if constexpr (K::kParts == 1)
+    std::conditional_t<STATS, char, typename M::Own> o;
+    if constexpr (!STATS)
       at_own<K, HD, VEC>(o, AtSource<K>{static_cast<const E*>(a.out), 0, a.out_cols, a.hd}, row0 + qw0, qc, n, lane);
     // the first tiles are on their way while D waits for the rows above
     auto load = [&](E* tile, int col, int k0, int wave) {
@@ -172,9 +179,9 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
       fetch(0, smem);
     }
     float D, lse2;
-    if constexpr (K::kParts > 1) {  // the statistics came with the parts
+    if constexpr (STATS) {
       const float* st = stat_part(a, at.g, qw0) + (lane & 31);
-      lse2 = q < len ? -st[0] : INFINITY;
+      lse2 = q < len ? sizeof(O) == 4 ? -st[0] : -st[0] * sl2 : INFINITY;
       D = q < len ? -st[32] : 0.f;
     } else {
       D = M::dot(dout.v[0], o.v[0]);
@@ -242,21 +249,17 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
   }
 }
 
+// dk and dv of block `block` of `blocks`.
 template <typename K, int HD, int KS, bool VEC>
-__global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_kv(const AttnTrain a) {
+__device__ __forceinline__ void backward_kv(const AttnTrain& a, int block, int blocks, char* smem, char* odd, float (*stat)[64],
+                                            float (*stat_odd)[64]) {
   typedef AtMma<K, HD> M;
   typedef typename K::E E;
   typedef typename K::O O;
   typedef AtPlan<K, HD, KS, VEC> P;
-  constexpr int kJoin = KS == 4 ? kJoinFloats<HD> * 4 : 0, kHalf = P::kBytes / 2;
-  // KS == 1: [Q, dO] tiles, and the same for odd steps; KS == 4: the waves' Q tiles, and their dO tiles
-  constexpr int kFirst = KS == 1 ? P::kBytes : kHalf > kJoin ? kHalf : kJoin;
-  __shared__ __align__(1024) char smem[kFirst], odd[KS == 4 ? kHalf : P::kBufs == 2 ? P::kBytes : 16];
-  constexpr int kStats = KS == 4 ? 4 : P::kParts;  // a buffer's 32-row parts: the tile's, or the waves'
-  __shared__ __align__(1024) float stat[kStats][64], stat_odd[KS == 4 ? 1 : kStats][64];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const AtBlock at = at_block(blockIdx.x, a.B * a.Hk, a.ragged);
+  const AtBlock at = at_block(block, blocks, a.B * a.Hk, a.ragged);
   const int b = at.g / a.Hk, kvh = at.g % a.Hk, group = a.H / a.Hk;
   const int k0 = at.blk * P::kOwn, len = at_len(a, b);
   const int kw0 = k0 + (KS == 1 ? 32 * w : 0), key = kw0 + (lane & 31);
@@ -411,23 +414,84 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_bac
   }
 }
 
+template <typename K, int HD, int KS, bool VEC>
+__global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O) == 4 ? 1 : 2) void k_attn_backward_q(
+    const AttnTrain a) {
+  typedef BackLds<K, HD, KS, VEC> L;
+  __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
+  backward_q<K, HD, KS, VEC, (K::kParts > 1)>(a, blockIdx.x, gridDim.x, smem, odd);
+}
+template <typename K, int HD, int KS, bool VEC>
+__global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_kv(const AttnTrain a) {
+  typedef BackLds<K, HD, KS, VEC> L;
+  __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
+  __shared__ __align__(1024) float stat[L::kStats][64], stat_odd[L::kStatsOdd][64];
+  backward_kv<K, HD, KS, VEC>(a, blockIdx.x, gridDim.x, smem, odd, stat, stat_odd);
+}
+// Both, where blocks are few: those of dk and dv first, which have more to do, and those of dq fill the CUs
+// that the last of them leave idle.
+template <typename K, int HD>
+__global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_both(const AttnTrain a, int kv_blocks) {
+  typedef BackLds<K, HD, 4, true> L;
+  __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
+  __shared__ __align__(1024) float stat[L::kStats][64], stat_odd[L::kStatsOdd][64];
+  if ((int)blockIdx.x < kv_blocks)
+    backward_kv<K, HD, 4, true>(a, blockIdx.x, kv_blocks, smem, odd, stat, stat_odd);
+  else
+    backward_q<K, HD, 4, true, true>(a, blockIdx.x - kv_blocks, gridDim.x - kv_blocks, smem, odd);
+}
+
+// The rows' statistics (stat_part), 8 lanes to a row of a head.  Those of parts past a length are not read.
+template <typename O>
+__global__ __launch_bounds__(256) void k_attn_stats(const AttnTrain a) {
+  constexpr int CE = 16 / sizeof(O);
+  const int j = threadIdx.x & 7, rows = (a.T + 31) & ~31;
+  const size_t n = (size_t)a.B * rows * a.H;
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) >> 3; i < n; i += (size_t)gridDim.x * 32) {
+    const int h = i % a.H, t = i / a.H % rows, b = i / a.H / rows;
+    const int len = a.ragged ? (a.lens_dev ? a.lens_dev[b] : a.lens[b]) : a.T;
+    const size_t row = ((size_t)b * a.T + t) * a.out_cols + (size_t)h * a.hd;
+    float D = 0.f;
+    for (int c = j; c * CE < a.hd && t < len; c += 8) {  // (hd is a multiple of CE)
+      typedef O oc __attribute__((ext_vector_type(CE)));
+      const oc x = *reinterpret_cast<const oc*>(static_cast<const O*>(a.dout) + row + c * CE);
+      const oc y = *reinterpret_cast<const oc*>(static_cast<const O*>(a.out) + row + c * CE);
+#pragma unroll
+      for (int e = 0; e < CE; e++) D = fmaf((float)x[e], (float)y[e], D);
+    }
+#pragma unroll
+    for (int s = 1; s < 8; s <<= 1) D += __shfl_xor(D, s, 64);
+    const size_t head = (size_t)b * a.H + h;
+    if (j == 0) {
+      float* st = stat_part(a, head, t) + t % 32;
+      st[0] = t < len ? -a.lse[head * a.T + t] * (sizeof(O) == 4 ? kLog2e : 1.f / a.scale) : -INFINITY;
+      st[32] = t < len ? -D : 0.f;
+    }
+  }
+}
+
 template <typename K, int HD, bool VEC>
 void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   const size_t wide = (size_t)((a.T + 127) / 128), narrow = (size_t)((a.T + 31) / 32);
   const size_t gq = (size_t)a.B * a.H, gk = (size_t)a.B * a.Hk;
-  bool few_q = at_few<K, HD>(wide * gq, cus), few_k = at_few<K, HD>(wide * gk, cus);
   if constexpr (VEC) {
-    if (few_q)
-      hipLaunchKernelGGL((k_attn_backward_q<K, HD, 4, VEC>), dim3((unsigned)(narrow * gq)), dim3(256), 0, st, a);
-  } else {
-    few_q = few_k = false;
+    if (at_few<K, HD>(wide * gq, cus)) {
+      if constexpr (K::kParts == 1) {
+        hipLaunchKernelGGL((k_attn_stats<typename K::O>), dim3((unsigned)(narrow * gq)), dim3(256), 0, st, a);
+      }
+      hipLaunchKernelGGL((k_attn_backward_both<K, HD>), dim3((unsigned)(narrow * (gq + gk))), dim3(256), 0, st, a,
+                         (int)(narrow * gk));
+      return;
+    }
   }
-  if (!few_q) hipLaunchKernelGGL((k_attn_backward_q<K, HD, 1, VEC>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_attn_backward_q<K, HD, 1, VEC>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
   if constexpr (VEC) {
-    if (few_k)
+    if (at_few<K, HD>(wide * gk, cus)) {
       hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 4, VEC>), dim3((unsigned)(narrow * gk)), dim3(256), 0, st, a);
+      return;
+    }
   }
-  if (!few_k) hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 1, VEC>), dim3((unsigned)(wide * gk)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 1, VEC>), dim3((unsigned)(wide * gk)), dim3(256), 0, st, a);
 }
 
 template <typename K, bool VEC>
