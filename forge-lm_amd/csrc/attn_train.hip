@@ -40,10 +40,13 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
   typedef typename K::O O;
   typedef AtPlan<K, HD, KS, VEC> P;
   constexpr int N = HD < 64 ? HD : 64;  // dims joined at a time
+  // V from memory to registers: a wave's own tile is read once, and its LDS is what a third block of the CU needs
+  // (4 x 512 rows, 12 heads of 64: 35.3 and 31.6 us)
+  constexpr bool kDirect = std::is_same_v<K, AtF32> && KS == 4 && HD <= 64;
   constexpr int kJoin = KS == 4 ? 4 * 32 * (N + 3) * 4 : 0, kHalf = P::kBytes / 2;
   // KS == 1: [K, V] tiles, and the same for odd steps; KS == 4: the waves' K tiles, and their V tiles
   constexpr int kFirst = KS == 1 ? P::kBytes : kHalf > kJoin ? kHalf : kJoin;
-  __shared__ __align__(1024) char smem[kFirst], odd[KS == 4 ? kHalf : P::kBufs == 2 ? P::kBytes : 16];
+  __shared__ __align__(1024) char smem[kFirst], odd[kDirect ? 16 : KS == 4 ? kHalf : P::kBufs == 2 ? P::kBytes : 16];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nqb = (a.T + P::kOwn - 1) / P::kOwn;
@@ -68,10 +71,10 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
     };
     // the 32 N keys from k0 on, tile rows r0 ..; the calls come where the K tile has been read for the last
     // time, and before the V tile is read
-    auto part = [&](auto nparts, int k0, const E* Ks, const E* Vs, int r0, auto&& k_read, auto&& v_wait) {
+    auto part = [&](auto nparts, int k0, const E* Ks, const auto& V, int r0, auto&& k_read, auto&& v_wait) {
       constexpr int N = decltype(nparts)::value;
       at_f32x16 s[N];
-      typename M::Cols vf[N];
+      std::conditional_t<kDirect, char, typename M::Cols> vf[N];
 #pragma unroll
       for (int i = 0; i < N; i++) {
         at_zero(s[i]);
@@ -79,8 +82,9 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
       }
       k_read();
       v_wait();
+      if constexpr (!kDirect)
 #pragma unroll
-      for (int i = 0; i < N; i++) vf[i] = M::load_cols(Vs, P::kSub, r0 + 32 * i, lane);
+        for (int i = 0; i < N; i++) vf[i] = M::load_cols(V, P::kSub, r0 + 32 * i, lane);
       const bool edge = N == 1 && k0 + 31 > qw0;  // the part crosses the diagonal
       if (edge) {
         const int left = q - k0 - 4 * (lane >> 5);  // at_row0 of the last key that the query sees
@@ -114,8 +118,11 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
           ls += s[i][r];
         }
       l += ls;
+      if constexpr (kDirect)
+        V.cols(o, s[0]);
+      else
 #pragma unroll
-      for (int i = 0; i < N; i++) M::cols(o, vf[i], s[i], lane);
+        for (int i = 0; i < N; i++) M::cols(o, vf[i], s[i], lane);
     };
     if constexpr (KS == 1) {
       auto fetch = [&](int kt, char* buf) {
@@ -136,6 +143,21 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
             part(at_int<1>, k0 + 32 * n, t, t + P::kTile, 32 * n, [] {}, [] {});
       };
       at_walk<P>((min(t0 + P::kOwn, len) - 1) / P::kRows + 1, smem, odd, fetch, compute);
+    } else if constexpr (kDirect) {
+      E* Ks = reinterpret_cast<E*>(smem) + w * P::kTile;
+      const int last = t0 / 32;
+      if (w <= last) load(Ks, kc, 32 * w, 0);
+      for (int p = w; p <= last; p += 4) {  // (past the last part nothing is in reach, and zeros arrive)
+        AtColsF32<HD> v;
+        v.load(x.rows(0, row0 + 32 * p, vc, min(32, len - 32 * p)), lane);
+        at_wait<16 * HD / 32>();
+        part(at_int<1>, 32 * p, Ks, v, 0,
+             [&] {
+               at_wait<-1>();
+               load(Ks, kc, 32 * (p + 4), 0);
+             },
+             [] {});
+      }
     } else {
       E *Ks = reinterpret_cast<E*>(smem) + w * P::kTile, *Vs = reinterpret_cast<E*>(odd) + w * P::kTile;
       const int last = t0 / 32;

@@ -262,6 +262,29 @@ struct AtMma<AtF32, HD> {
   }
 };
 
+// fp32: 32 rows of m as the operand of `cols`, from memory to registers; zeros past either end of m.
+template <int HD>
+struct AtColsF32 {
+  float v[16][HD / 32];
+  __device__ __forceinline__ void load(const AtRows<float>& m, int lane) {
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; dt++) {
+      const int d = dt * 32 + (lane & 31);
+      int at = d < m.hd ? 4 * (lane >> 5) * m.stride + 4 * d : 0x7ffffff0;
+      asm volatile("" : "+v"(at));  // (or all the loads' offsets are kept in registers from one part to the next)
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        v[r][dt] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(m.rsrc, at + at_row0(r) * m.stride, 0, 0));
+    }
+  }
+  __device__ __forceinline__ void cols(at_f32x16 (&acc)[HD / 32], const at_f32x16& w) const {
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; dt++) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][dt], w[r], acc[dt], 0, 0, 0);
+  }
+};
+
 // A matrix in parts: the rows of each, `part` elements (of the whole matrix) apart.
 template <typename K>
 struct AtSource {

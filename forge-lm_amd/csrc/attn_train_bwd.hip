@@ -428,17 +428,18 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_bac
   __shared__ __align__(1024) float stat[L::kStats][64], stat_odd[L::kStatsOdd][64];
   backward_kv<K, HD, KS, VEC>(a, blockIdx.x, gridDim.x, smem, odd, stat, stat_odd);
 }
-// Both, where blocks are few: those of dk and dv first, which have more to do, and those of dq fill the CUs
-// that the last of them leave idle.
-template <typename K, int HD>
+// Both in one launch: the blocks of dk and dv first, which have more to do, and those of dq fill the CUs that
+// the last of them leave idle.
+template <typename K, int HD, int QS, int KS>
 __global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_both(const AttnTrain a, int kv_blocks) {
-  typedef BackLds<K, HD, 4, true> L;
-  __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
+  typedef BackLds<K, HD, KS, true> L;
+  typedef BackLds<K, HD, QS, true> Q;
+  __shared__ __align__(1024) char smem[L::kFirst > Q::kFirst ? L::kFirst : Q::kFirst], odd[L::kOdd > Q::kOdd ? L::kOdd : Q::kOdd];
   __shared__ __align__(1024) float stat[L::kStats][64], stat_odd[L::kStatsOdd][64];
   if ((int)blockIdx.x < kv_blocks)
-    backward_kv<K, HD, 4, true>(a, blockIdx.x, kv_blocks, smem, odd, stat, stat_odd);
+    backward_kv<K, HD, KS, true>(a, blockIdx.x, kv_blocks, smem, odd, stat, stat_odd);
   else
-    backward_q<K, HD, 4, true, true>(a, blockIdx.x - kv_blocks, gridDim.x - kv_blocks, smem, odd);
+    backward_q<K, HD, QS, true, true>(a, blockIdx.x - kv_blocks, gridDim.x - kv_blocks, smem, odd);
 }
 
 // The rows' statistics (stat_part), 8 lanes to a row of a head.  Those of parts past a length are not read.
@@ -474,24 +475,53 @@ template <typename K, int HD, bool VEC>
 void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   const size_t wide = (size_t)((a.T + 127) / 128), narrow = (size_t)((a.T + 31) / 32);
   const size_t gq = (size_t)a.B * a.H, gk = (size_t)a.B * a.Hk;
-  if constexpr (VEC) {
-    if (at_few<K, HD>(wide * gq, cus)) {
-      if constexpr (K::kParts == 1) {
-        hipLaunchKernelGGL((k_attn_stats<typename K::O>), dim3((unsigned)(narrow * gq)), dim3(256), 0, st, a);
-      }
-      hipLaunchKernelGGL((k_attn_backward_both<K, HD>), dim3((unsigned)(narrow * (gq + gk))), dim3(256), 0, st, a,
-                         (int)(narrow * gk));
+  // dq in blocks of 128 rows, and then dk and dv
+  auto in_turn = [&](auto ks) {
+    constexpr int KS = decltype(ks)::value;
+    hipLaunchKernelGGL((k_attn_backward_q<K, HD, 1, VEC>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_attn_backward_kv<K, HD, KS, VEC>), dim3((unsigned)((KS == 4 ? narrow : wide) * gk)), dim3(256), 0, st, a);
+  };
+  auto together = [&](auto qs, auto ks) {
+    constexpr int QS = decltype(qs)::value, KS = decltype(ks)::value;
+    const size_t kv = (KS == 4 ? narrow : wide) * gk, q = (QS == 4 ? narrow : wide) * gq;
+    if constexpr (K::kParts == 1)
+      hipLaunchKernelGGL((k_attn_stats<typename K::O>), dim3((unsigned)(narrow * gq)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_attn_backward_both<K, HD, QS, KS>), dim3((unsigned)(kv + q)), dim3(256), 0, st, a, (int)kv);
+  };
+  if constexpr (!VEC) {
+    in_turn(at_int<1>);
+  } else {
+    const bool few_q = at_few<K, HD>(wide * gq, cus), few_k = at_few<K, HD>(wide * gk, cus);
+    if (few_q) {
+      together(at_int<4>, at_int<4>);
       return;
     }
-  }
-  hipLaunchKernelGGL((k_attn_backward_q<K, HD, 1, VEC>), dim3((unsigned)(wide * gq)), dim3(256), 0, st, a);
-  if constexpr (VEC) {
-    if (at_few<K, HD>(wide * gk, cus)) {
-      hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 4, VEC>), dim3((unsigned)(narrow * gk)), dim3(256), 0, st, a);
-      return;
+    // One launch costs the statistics' (3 to 5 us), and dq the waves that the registers of dk and dv leave no
+    // room for; it saves what the CUs idle while the last blocks of dk and dv end, which are up to T / 128 times
+    // as long as the first.  us in turn and in one, blocks of dk and dv by sequences x rows:
+    //   bf16, 12 heads of 64  384 (4 x 1024) 57 and 46, 384 (1 x 4096) 182 and 129, 768 (8 x 1024) 78 and 80
+    //   bf16, 16 heads of 128  256 (2 x 4096, 4 of k and v) 761 and 652, 384 (8 x 300) 43 and 49; in blocks of 32
+    //                  (4 x 1333, 4 of k and v) 207 and 223
+    //   fp32, 12 heads of 64  384 (4 x 1024) 235 and 222, 768 (8 x 1024) 386 and 412; not in parts, where dq has
+    //                  no more waves either, 768 (32 x 256) 189 and 174
+    if constexpr (std::is_same_v<K, AtF32>) {
+      few_k ? together(at_int<1>, at_int<4>) : together(at_int<1>, at_int<1>);
+    } else if constexpr (HD <= 64) {
+      if (few_k)
+        together(at_int<1>, at_int<4>);
+      else if (wide * gk < 2 * (size_t)cus)
+        together(at_int<1>, at_int<1>);
+      else
+        in_turn(at_int<1>);
+    } else {
+      if (few_k)
+        in_turn(at_int<4>);
+      else if (wide * gk <= (size_t)cus)
+        together(at_int<1>, at_int<1>);
+      else
+        in_turn(at_int<1>);
     }
   }
-  hipLaunchKernelGGL((k_attn_backward_kv<K, HD, 1, VEC>), dim3((unsigned)(wide * gk)), dim3(256), 0, st, a);
 }
 
 template <typename K, bool VEC>

@@ -189,6 +189,17 @@ def test_attention_many_blocks(fhp, be, hd, Hk, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,H,Hk,hd,dtype", [
+    (16, 133, 16, 4, 128, "bf16"), (16, 133, 16, 8, 128, "bf16"),  # blocks of keys: few, as many as CUs
+    (16, 133, 16, 8, 64, "bf16"), (8, 260, 32, 32, 32, "bf16"), (16, 133, 16, 8, 128, "f32"), (16, 133, 20, 20, 128, "f32"),
+    (16, 260, 16, 16, 32, "f32"), (16, 260, 16, 2, 64, "f32"), (8, 260, 24, 12, 48, "f32"),  # in three parts
+])
+def test_attention_blocks_of_queries_and_keys(fhp, be, B, T, H, Hk, hd, dtype):
+    # dq, dk and dv in one launch or in turn, in blocks of 32 and of 128 rows
+    attention_case(fhp, be, B, T, H, Hk, hd, dtype, seed=hd + H)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_many_blocks_unaligned(fhp, be, dtype):
     attention_case(fhp, be, 16, 133, 16, 16, 25, dtype, seed=25, more=1)
