@@ -286,11 +286,22 @@ __global__ __launch_bounds__(256) void k_attn_split(const AttnTrain a, const flo
   }
 }
 
+// Whether `blocks` blocks of 128 rows are so few that KS 4 pays: a wave's chain of steps is a quarter as long,
+// and every tile is fetched for 32 rows instead of 128.  us with KS 1 and KS 4, 12 heads of 64 but where said:
+//   bf16  192 blocks (2 x 1024) 20 and 16, 256 (4 x 1024, 8 heads) 21 and 23, 384 (4 x 1024) 24 and 29
+//   fp32  192 blocks 87 and 53, 384 100 and 89, 768 153 and 165; heads of 128: 256 blocks (2 x 2000, 8 heads) 291
+//         and 228, 384 (8 x 300, 16 heads) 73 and 98
+template <typename K, int HD>
+bool few_blocks(size_t blocks, int cus) {
+  const size_t quarters = std::is_same_v<K, AtF32> ? HD > 64 ? 5 : 8 : 4;  // of the CUs
+  return 4 * blocks < quarters * cus;
+}
+
 template <typename K, int HD, bool VEC>
 void forward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   const size_t g = (size_t)a.B * a.H, wide = (size_t)((a.T + 127) / 128) * g, narrow = (size_t)((a.T + 31) / 32) * g;
   if constexpr (VEC && K::kParts == 1) {  // (parts: where blocks are many, attn_train_split)
-    if (at_few<K, HD>(wide, cus)) {
+    if (few_blocks<K, HD>(wide, cus)) {
       hipLaunchKernelGGL((k_attn_forward<K, HD, 4, VEC>), dim3((unsigned)narrow), dim3(256), 0, st, a);
       return;
     }

@@ -426,20 +426,6 @@ struct AtPlan {
                               : 64 * HD * (int)sizeof(O) <= kBytes ? 16 : 0;
 };
 
-// Whether `blocks` blocks of 128 rows are so few that KS 4 pays: a wave's chain of steps is a quarter as long,
-// and every tile is fetched for 32 rows instead of 128.  us with KS 1 and KS 4, 12 heads of 64 but where said:
-//   bf16 forward   192 blocks (2 x 1024) 20 and 16, 256 (4 x 1024, 8 heads) 21 and 23, 384 (4 x 1024) 24 and 29
-//   bf16 backward  192 blocks 48 and 38, 384 57 and 67, 768 (8 x 1024) 77 and 129
-//   fp32 forward   192 blocks 87 and 53, 384 100 and 89, 768 153 and 165; heads of 128: 256 blocks (2 x 2000,
-//                  8 heads) 291 and 228, 384 (8 x 300, 16 heads) 73 and 98
-//   fp32 backward  96 blocks (2 x 512) 132 and 60, 288 (8 x 333, heads of 40) 118 and 99
-//   in parts, backward  192 blocks 175 and 144, 384 210 and 260
-template <typename K, int HD>
-bool at_few(size_t blocks, int cus) {
-  const size_t quarters = std::is_same_v<K, AtF32> ? HD > 64 ? 5 : 8 : 4;  // of the CUs
-  return 4 * blocks < quarters * cus;
-}
-
 // A tile of rows `row` .. of x: by all four waves of the block (KS == 1), or by this wave alone.
 template <typename K, int HD, int KS, bool VEC>
 __device__ __forceinline__ void at_load(typename K::E* tile, const AtSource<K>& x, size_t row, size_t col, int rows, int w,

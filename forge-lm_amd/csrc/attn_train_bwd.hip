@@ -471,6 +471,25 @@ __global__ __launch_bounds__(256) void k_attn_stats(const AttnTrain a) {
   }
 }
 
+// Whether `blocks` blocks of 128 rows, which walk the rows of `heads` heads, are so few that KS 4 pays (chains a
+// quarter as long, tiles fetched for 32 rows instead of 128); fewer where T is so short that a block of 128 rows
+// has no chain.  us with KS 1 and KS 4, dq, dk and dv in one launch:
+//   bf16, 12 heads of 64   96 blocks (1 x 1024) 29 and 25, (2 x 512) 19 and 21; 144 (3 x 512) 21 and 28; 192
+//                          (2 x 1024) 34 and 39, (1 x 2048) 58 and 56; heads of 32: 128 (2 x 2048, 4 heads) 38 and
+//                          24; heads of 128: 96 (1 x 700, 16 heads) 35 and 47
+//   in parts               96 (1 x 1024) 110 and 88, 192 (2 x 1024) 129 and 155, 240 (1 x 2500) 271 and 309; heads
+//                          of 32: 128 (2 x 2048, 4 heads) 130 and 82
+//   fp32                   192 (4 x 512) 118 and 95, (8 x 256) 71 and 67, (16 x 128) 43 and 51; 288 (12 x 256) 80
+//                          and 98; heads of 128: 128 (1 x 1000, 16 heads) 283 and 215, (8 x 128) 54 and 82
+//   dk and dv where 4 heads share k and v (dq KS 1): bf16 64 blocks (4 x 1024, 8 heads of 64) 90 and 43, 176
+//                          (4 x 1333, 16 heads of 128) 212 and 205
+template <typename K, int HD>
+bool few_blocks(size_t blocks, int T, int heads, int cus) {
+  const int q = std::is_same_v<K, AtF32> ? HD > 64 ? 3 : 4 : HD > 64 ? 1 : HD > 32 ? 2 : 3;  // quarters of the CUs
+  const int quarters = heads < q ? q : heads > 4 ? 4 : heads;
+  return 4 * 256 * blocks < (size_t)quarters * cus * (T < 256 ? T : 256);
+}
+
 template <typename K, int HD, bool VEC>
 void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   const size_t wide = (size_t)((a.T + 127) / 128), narrow = (size_t)((a.T + 31) / 32);
@@ -491,7 +510,8 @@ void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   if constexpr (!VEC) {
     in_turn(at_int<1>);
   } else {
-    const bool few_q = at_few<K, HD>(wide * gq, cus), few_k = at_few<K, HD>(wide * gk, cus);
+    const bool few_q = few_blocks<K, HD>(wide * gq, a.T, 1, cus);
+    const bool few_k = few_q || few_blocks<K, HD>(wide * gk, a.T, a.H / a.Hk, cus);
     if (few_q) {
       together(at_int<4>, at_int<4>);
       return;
@@ -501,7 +521,7 @@ void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
     // as long as the first.  us in turn and in one, blocks of dk and dv by sequences x rows:
     //   bf16, 12 heads of 64  384 (4 x 1024) 57 and 46, 384 (1 x 4096) 182 and 129, 768 (8 x 1024) 78 and 80
     //   bf16, 16 heads of 128  256 (2 x 4096, 4 of k and v) 761 and 652, 384 (8 x 300) 43 and 49; in blocks of 32
-    //                  (4 x 1333, 4 of k and v) 207 and 223
+    //                  and dq in 704 (4 x 1333, 4 of k and v) 205 and 226, in 192 (4 x 700, 8 heads, 2) 69 and 53
     //   fp32, 12 heads of 64  384 (4 x 1024) 235 and 222, 768 (8 x 1024) 386 and 412; not in parts, where dq has
     //                  no more waves either, 768 (32 x 256) 189 and 174
     if constexpr (std::is_same_v<K, AtF32>) {
@@ -515,7 +535,7 @@ void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
         in_turn(at_int<1>);
     } else {
       if (few_k)
-        in_turn(at_int<4>);
+        wide * gq <= 2 * (size_t)cus ? together(at_int<1>, at_int<4>) : in_turn(at_int<4>);
       else if (wide * gk <= (size_t)cus)
         together(at_int<1>, at_int<1>);
       else
