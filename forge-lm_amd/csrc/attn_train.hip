@@ -233,15 +233,29 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
   }
 }
 
-// The parts of NH heads of hd columns each of x's rows (x_cols apart): rows of NH * hp columns of bf16, hp
-// = hd to the next 8, zeros past hd; the three parts `part` elements apart.  A power of two of lanes, 1 <<
-// lg >= hp / 8, takes a row of a head.  Where o is not null, x is do and the rows' statistics are written
-// too (stat_part).  Rows past a sequence's length are not read and not written.
-__global__ __launch_bounds__(256) void k_attn_split(const AttnTrain a, const float* __restrict__ x, int x_cols, int NH,
-                                                    __bf16* __restrict__ parts, size_t part, int lg, const float* __restrict__ o) {
+// A matrix and where its parts go.
+struct Split {
+  const float* x;
+  int cols, NH;  // columns of x's rows, heads
+  __bf16* parts;
+  size_t part;     // elements of one part
+  const float* o;  // not null: x is do, and the rows' statistics are written too (stat_part)
+  int blocks;
+};
+// The parts of NH heads of hd columns each of x's rows: rows of NH * hp columns of bf16, hp = hd to the next 8,
+// zeros past hd; the three parts `part` elements apart.  A power of two of lanes, 1 << lg >= hp / 8, takes a
+// row of a head.  Rows past a sequence's length are not read and not written.  The first blocks take s0, the
+// others s1.
+__global__ __launch_bounds__(256) void k_attn_split(const AttnTrain a, const Split s0, const Split s1, int lg) {
+  const bool second = (int)blockIdx.x >= s0.blocks;
+  const float *x = second ? s1.x : s0.x, *o = second ? s1.o : s0.o;
+  const int x_cols = second ? s1.cols : s0.cols, NH = second ? s1.NH : s0.NH;
+  __bf16* parts = second ? s1.parts : s0.parts;
+  const size_t part = second ? s1.part : s0.part;
+  const int block = blockIdx.x - (second ? s0.blocks : 0), blocks = second ? s1.blocks : s0.blocks;
   const int hp = a.in_hd, j = threadIdx.x & ((1 << lg) - 1), rows = a.T + 31 & ~31;
   const size_t n = (size_t)a.B * rows * NH;
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) >> lg; i < n; i += (size_t)gridDim.x * (256 >> lg)) {
+  for (size_t i = ((size_t)block * 256 + threadIdx.x) >> lg; i < n; i += (size_t)blocks * (256 >> lg)) {
     const int h = i % NH, t = i / NH % rows, b = i / NH / rows, len = a.ragged ? (a.lens_dev ? a.lens_dev[b] : a.lens[b]) : a.T;
     const size_t row = (size_t)b * a.T + t;
     float v[8] = {}, D = 0.f;
@@ -338,16 +352,16 @@ size_t stat_floats(const AttnTrain& a) { return (size_t)a.B * a.H * ((a.T + 31) 
 }  // namespace
 
 // Whether fp32 tensors are multiplied in three bf16 parts, which takes 3/8 of the matrix cores' time and a launch
-// (backward: two) that writes the parts.  12 heads of 64, us with the fp32 instruction and in parts:
+// that writes the parts.  12 heads of 64, us with the fp32 instruction and in parts:
 //   forward   8 x 512 58 and 58, 16 x 512 90 and 91, 32 x 256 61 and 76; 4 x 1024 89 and 81, 8 x 1024 153 and
 //             121, 2 x 2048 146 and 122; in few blocks 2 x 1024 53 and 70, 1 x 2048 84 and 93
-//   backward  2 x 512 60 and 76, 4 x 512 100 and 108, 32 x 256 189 and 199; 8 x 512 176 and 147, 1 x 1024
-//             105 and 89, 4 x 1024 266 and 210, 8 x 1024 470 and 342, 1 x 2048 252 and 205
+//   backward  2 x 512 60 and 68, 2 x 700 85 and 91, 16 x 256 103 and 108; 4 x 512 96 and 84, 8 x 512 176 and 147,
+//             1 x 1024 105 and 89, 4 x 1024 266 and 210, 8 x 1024 470 and 342, 1 x 2048 252 and 205
 // Heads above 64 would not keep their three parts in registers.
 bool attn_train_split(const AttnTrain& a, bool backward, int cus) {
   const size_t blocks = (size_t)a.B * a.H * ((a.T + 127) / 128);
   if (a.hd > 64 || !whole_chunks(a, 4)) return false;
-  return backward ? a.T >= 1024 || (a.T > 256 && blocks >= (size_t)cus) : a.T > 512 && blocks > (size_t)cus;
+  return backward ? a.T >= 1024 || (a.T > 256 && 4 * blocks >= 3 * (size_t)cus) : a.T > 512 && blocks > (size_t)cus;
 }
 
 size_t attn_train_scratch(const AttnTrain& a, bool bf16, bool backward, bool split, int cus) {
@@ -375,13 +389,15 @@ hipError_t attn_train_inputs(hipStream_t st, AttnTrain& a, bool bf16, bool backw
   a.in = parts, a.in_do = do_parts;
   int lg = 0;
   while ((8 << lg) < a.in_hd) lg++;
-  auto launch = [&](const float* x, int cols, int heads, __bf16* to, size_t part, const float* o) {
+  auto split_of = [&](const void* x, int cols, int heads, __bf16* to, size_t part, const void* o) {
     const size_t n = ((size_t)a.B * ((a.T + 31) / 32 * 32) * heads << lg) / 256 + 1;
-    hipLaunchKernelGGL(k_attn_split, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a, x, cols, heads, to, part, lg, o);
+    return Split{static_cast<const float*>(x), cols, heads, to, part, static_cast<const float*>(o),
+                 (int)(n < 65536 ? n : 65536)};
   };
-  launch(static_cast<const float*>(a.qkv), a.qkv_cols, a.H + 2 * a.Hk, parts, a.in_part, nullptr);
-  if (backward)
-    launch(static_cast<const float*>(a.dout), a.out_cols, a.H, do_parts, a.do_part, static_cast<const float*>(a.out));
+  const Split s0 = split_of(a.qkv, a.qkv_cols, a.H + 2 * a.Hk, parts, a.in_part, nullptr);
+  Split s1{};
+  if (backward) s1 = split_of(a.dout, a.out_cols, a.H, do_parts, a.do_part, a.out);
+  hipLaunchKernelGGL(k_attn_split, dim3((unsigned)(s0.blocks + s1.blocks)), dim3(256), 0, st, a, s0, s1, lg);
   return hipGetLastError();
 }
 
