@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nqb = (a.T + P::kOwn - 1) / P::kOwn;
-  const AtBlock at = at_block(blockIdx.x, gridDim.x, a.B * a.H, a.ragged);
+  const AtBlock at = at_block(blockIdx.x, gridDim.x, 0, a.B * a.H, a.ragged);
   const int b = at.g / a.H, h = at.g % a.H, kvh = h / (a.H / a.Hk);
   const int t0 = (nqb - 1 - at.blk) * P::kOwn, len = at_len(a, b);
   const int qw0 = t0 + (KS == 1 ? 32 * w : 0), q = qw0 + (lane & 31);

@@ -526,22 +526,26 @@ __device__ __forceinline__ void at_put_row(O* row, const float (&acc)[N], float 
 // Block -> (block of the axis, group = sequence * heads + head) of a causal launch over nblk * G
 // blocks; block 0 of the axis is the one with the most work, and is started first.  Workgroups reach
 // the 8 XCDs round-robin.  Sequences of one length: when 8 divides G, an XCD takes whole neighbouring
-// groups, so that what their blocks share is fetched into its L2 only; every other 32 of its blocks (one for
-// each of its CUs) come in reverse, so that a CU's blocks add up to the same (dq of 8 x 1024 rows, three
-// blocks to a CU: 32.1 -> 30.5 us).  Sequences of their own lengths:
+// groups, so that what their blocks share is fetched into its L2 only.  Every other 32 of its blocks (256 of the
+// launch's), one for each CU, come in reverse, so that a CU's blocks add up to the same (dq of 8 x 1024 rows, three
+// blocks to a CU: 32.1 -> 30.5 us); `before`: blocks that the launch has before these.  Sequences of their own lengths:
 // a group's blocks go to all XCDs in turn, which evens out what long ones cost (4 x up to 1333 rows, 16
 // heads of 128, dq: 60 us with groups kept together, an XCD idle for half of it).
 struct AtBlock {
   int blk, g;
 };
-__device__ __forceinline__ AtBlock at_block(int L, int blocks, int G, int ragged) {
-  if (!ragged && G % 8 == 0) {
-    const int gx = G / 8, i = L >> 3, first = i & ~31, n = min(32, (blocks >> 3) - first);
-    const int s = i & 32 ? first + n - 1 - (i - first) : i;
-    return {s / gx, (L & 7) * gx + s % gx};
+__device__ __forceinline__ AtBlock at_block(int L, int blocks, int before, int G, int ragged) {
+  if (ragged) {
+    const int blk = L / G, i = L % G;
+    return {blk, G % 2 == 0 ? (i + blk) % G : i};
   }
-  const int blk = L / G, i = L % G;
-  return {blk, ragged && G % 2 == 0 ? (i + blk) % G : i};
+  const bool grouped = G % 8 == 0;
+  // place among the blocks of the XCD, or of the launch; 1 << lg of them are one to a CU
+  const int i = grouped ? L >> 3 : L, n = grouped ? blocks >> 3 : blocks, off = grouped ? before >> 3 : before;
+  const int lg = grouped ? 5 : 8, turn = (i + off) >> lg;
+  const int first = max(0, (turn << lg) - off), last = min(n, ((turn + 1) << lg) - off) - 1;
+  const int s = turn & 1 ? first + last - i : i, per = grouped ? G / 8 : G;
+  return {s / per, grouped ? (L & 7) * per + s % per : s % per};
 }
 
 // q's columns of a matrix that a kernel reads (its k and v follow), and do's.

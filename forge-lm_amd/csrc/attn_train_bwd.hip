@@ -130,7 +130,7 @@ struct BackLds {
 
 // dq of block `block` of `blocks`.  STATS: the statistics are there; else this computes them for the other kernel.
 template <typename K, int HD, int KS, bool VEC, bool STATS>
-__device__ __forceinline__ void backward_q(const AttnTrain& a, int block, int blocks, char* smem, char* odd) {
+__device__ __forceinline__ void backward_q(const AttnTrain& a, int block, int blocks, int before, char* smem, char* odd) {
   typedef AtMma<K, HD> M;
   typedef typename K::E E;
   typedef typename K::O O;
@@ -138,7 +138,7 @@ __device__ __forceinline__ void backward_q(const AttnTrain& a, int block, int bl
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nqb = (a.T + P::kOwn - 1) / P::kOwn;
-  const AtBlock at = at_block(block, blocks, a.B * a.H, a.ragged);
+  const AtBlock at = at_block(block, blocks, before, a.B * a.H, a.ragged);
   const int b = at.g / a.H, h = at.g % a.H, kvh = h / (a.H / a.Hk);
   const int t0 = (nqb - 1 - at.blk) * P::kOwn, len = at_len(a, b);
   const int qw0 = t0 + (KS == 1 ? 32 * w : 0), q = qw0 + (lane & 31);
@@ -259,7 +259,7 @@ __device__ __forceinline__ void backward_kv(const AttnTrain& a, int block, int b
   typedef AtPlan<K, HD, KS, VEC> P;
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const AtBlock at = at_block(block, blocks, a.B * a.Hk, a.ragged);
+  const AtBlock at = at_block(block, blocks, 0, a.B * a.Hk, a.ragged);
   const int b = at.g / a.Hk, kvh = at.g % a.Hk, group = a.H / a.Hk;
   const int k0 = at.blk * P::kOwn, len = at_len(a, b);
   const int kw0 = k0 + (KS == 1 ? 32 * w : 0), key = kw0 + (lane & 31);
@@ -419,10 +419,14 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O)
     const AttnTrain a) {
   typedef BackLds<K, HD, KS, VEC> L;
   __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
-  backward_q<K, HD, KS, VEC, (K::kParts > 1)>(a, blockIdx.x, gridDim.x, smem, odd);
+  backward_q<K, HD, KS, VEC, (K::kParts > 1)>(a, blockIdx.x, gridDim.x, 0, smem, odd);
 }
+// Waves of dk and dv that a SIMD's registers hold at least (heads of 128, and parts of 64 where LDS has no room
+// for more: one)
+template <typename K, int HD, int KS>
+constexpr int kWaves = HD > 64 || (HD > 32 && K::kParts > 1 && KS == 4) ? 1 : 2;
 template <typename K, int HD, int KS, bool VEC>
-__global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_kv(const AttnTrain a) {
+__global__ __launch_bounds__(256, (kWaves<K, HD, KS>)) void k_attn_backward_kv(const AttnTrain a) {
   typedef BackLds<K, HD, KS, VEC> L;
   __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
   __shared__ __align__(1024) float stat[L::kStats][64], stat_odd[L::kStatsOdd][64];
@@ -431,7 +435,7 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_bac
 // Both in one launch: the blocks of dk and dv first, which have more to do, and those of dq fill the CUs that
 // the last of them leave idle.
 template <typename K, int HD, int QS, int KS>
-__global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_backward_both(const AttnTrain a, int kv_blocks) {
+__global__ __launch_bounds__(256, (kWaves<K, HD, KS>)) void k_attn_backward_both(const AttnTrain a, int kv_blocks) {
   typedef BackLds<K, HD, KS, true> L;
   typedef BackLds<K, HD, QS, true> Q;
   __shared__ __align__(1024) char smem[L::kFirst > Q::kFirst ? L::kFirst : Q::kFirst], odd[L::kOdd > Q::kOdd ? L::kOdd : Q::kOdd];
@@ -439,7 +443,7 @@ __global__ __launch_bounds__(256, K::kParts * HD >= 128 ? 1 : 2) void k_attn_bac
   if ((int)blockIdx.x < kv_blocks)
     backward_kv<K, HD, KS, true>(a, blockIdx.x, kv_blocks, smem, odd, stat, stat_odd);
   else
-    backward_q<K, HD, QS, true, true>(a, blockIdx.x - kv_blocks, gridDim.x - kv_blocks, smem, odd);
+    backward_q<K, HD, QS, true, true>(a, blockIdx.x - kv_blocks, gridDim.x - kv_blocks, kWaves<K, HD, KS> > 1 ? kv_blocks : 0, smem, odd);
 }
 
 // The rows' statistics (stat_part), 8 lanes to a row of a head.  Those of parts past a length are not read.
