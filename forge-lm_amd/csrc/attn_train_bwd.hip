@@ -3,10 +3,12 @@
 //
 //   p_ij = exp(scale q_i . k_j - lse_i)   D_i = do_i . o_i        ds_ij = p_ij (do_i . v_j - D_i)
 //   dv_j = sum_i p_ij do_i                dq_i = scale sum_j ds_ij k_j   dk_j = scale sum_i ds_ij q_i
-// One kernel takes blocks of queries and walks the keys (dq, and D for the other), one takes blocks of
-// keys and walks the queries of every head that shares them (dk, dv).  The scores and dP are computed in
-// both, 14 hd operations a visible pair where 10 would do, so that every gradient is summed by one
-// block in a fixed order: no atomics, the same bits on every run.
+// Blocks of queries walk the keys (dq), blocks of keys the queries of every head that shares them (dk, dv),
+// in one launch or in turn (backward_hd).  The scores and dP are computed in both, 14 hd operations a visible
+// pair where 10 would do, so that every gradient is summed by one block in a fixed order: no atomics, the same
+// bits on every run.  Bound by the matrix cores, the exponentials and products of a part beside them, and the
+// chain of the longest blocks.  Measured, 12 heads of 64 (of the 14 hd operations): fp32 4 x 512 rows 69 us
+// (82 TFLOP/s), 1 x 2500 238 us (141), bf16 8 x 1024 66 us (684).
 #include "attn_train.hpp"
 
 #include <math.h>
@@ -415,11 +417,10 @@ __device__ __forceinline__ void backward_kv(const AttnTrain& a, int block, int b
 }
 
 template <typename K, int HD, int KS, bool VEC>
-__global__ __launch_bounds__(256, K::kParts * HD >= 128 && sizeof(typename K::O) == 4 ? 1 : 2) void k_attn_backward_q(
-    const AttnTrain a) {
+__global__ __launch_bounds__(256, HD > 64 && sizeof(typename K::O) == 4 ? 1 : 2) void k_attn_backward_q(const AttnTrain a) {
   typedef BackLds<K, HD, KS, VEC> L;
   __shared__ __align__(1024) char smem[L::kFirst], odd[L::kOdd];
-  backward_q<K, HD, KS, VEC, (K::kParts > 1)>(a, blockIdx.x, gridDim.x, 0, smem, odd);
+  backward_q<K, HD, KS, VEC, false>(a, blockIdx.x, gridDim.x, 0, smem, odd);
 }
 // Waves of dk and dv that a SIMD's registers hold at least (heads of 128, and parts of 64 where LDS has no room
 // for more: one)
@@ -520,15 +521,14 @@ void backward_hd(hipStream_t st, const AttnTrain& a, int cus) {
       together(at_int<4>, at_int<4>);
       return;
     }
-    // One launch costs the statistics' (3 to 5 us), and dq the waves that the registers of dk and dv leave no
-    // room for; it saves what the CUs idle while the last blocks of dk and dv end, which are up to T / 128 times
-    // as long as the first.  us in turn and in one, blocks of dk and dv by sequences x rows:
-    //   bf16, 12 heads of 64  384 (4 x 1024) 57 and 46, 384 (1 x 4096) 182 and 129, 768 (8 x 1024) 78 and 80
+    // One launch costs the statistics' (3 to 5 us; with parts they come anyway), and bf16's dq the waves that the
+    // registers of dk and dv leave no room for; it saves what the CUs idle while the last blocks of dk and dv end,
+    // which are up to T / 128 times as long as the first.  us in turn and in one, by blocks of dk and dv:
+    //   bf16, 12 heads of 64  384 (4 x 1024) 57 and 46, 384 (1 x 4096) 182 and 129, 768 (8 x 1024) 77 and 83
     //   bf16, 16 heads of 128  256 (2 x 4096, 4 of k and v) 761 and 652, 384 (8 x 300) 43 and 49; in blocks of 32
     //                  and dq in 704 (4 x 1333, 4 of k and v) 205 and 226, in 192 (4 x 700, 8 heads, 2) 69 and 53
-    //   fp32, 12 heads of 64  384 (4 x 1024) 235 and 222, 768 (8 x 1024) 386 and 412; not in parts, where dq has
-    //                  no more waves either, 768 (32 x 256) 189 and 174
-    if constexpr (std::is_same_v<K, AtF32>) {
+    //   fp32, 12 heads of 64  768 (32 x 256) 189 and 174; in parts, 768 (16 x 512) 233 and 218, (8 x 1024) 336 and 318
+    if constexpr (!std::is_same_v<K, AtBf16>) {
       few_k ? together(at_int<1>, at_int<4>) : together(at_int<1>, at_int<1>);
     } else if constexpr (HD <= 64) {
       if (few_k)
