@@ -341,7 +341,11 @@ int fh_op_adamw_step(fh_context* ctx, void* w, const void* g, void* m, void* v, 
  * row's sum of exp(scale * score), which the backward pass takes in place of the probabilities.
  * lengths (host, or NULL: all T): the first lengths[b] rows of sequence b count; out rows past them are
  * zeros and their lse -infinity, and their q, k, v are not read.  out and lse must not overlap qkv; the
- * other columns of out rows are left as they are.  scale: finite and positive. */
+ * other columns of out rows are left as they are.  scale: finite and positive.
+ * A row's out and lse depend on no later row, whatever that holds (NaN, infinities); in the backward pass
+ * a row's dq depends on no later row, and what a row's q and dout hold reaches dk and dv of no later row.
+ * Long fp32 calls multiply each value as three bf16 parts, as exact as fp32 products; there an
+ * infinity in a row that is seen may come out as NaN. */
 int fh_op_attention_forward(fh_context* ctx, const void* qkv, int qkv_cols, void* out, int out_cols, float* lse,
                             const int32_t* lengths, int batch, int T, int n_heads, int n_kv_heads, int head_dim,
                             float scale, int dtype);
