@@ -345,9 +345,11 @@ bool whole_chunks(const AttnTrain& a, int esize) {
 
 }  // namespace
 
+// (of the launches, the largest has a block for every 32 rows of every head of q and of k and v: below 2^24)
 bool attn_train_fits(const AttnTrain& a) {
-  return a.B > 0 && a.T > 0 && a.Hk > 0 && a.H > 0 && a.H % a.Hk == 0 && a.hd > 0 && a.hd <= kAttnTrainHead &&
-         a.T <= 1 << 24 && a.qkv_cols <= 1 << 20 && a.out_cols <= 1 << 20 && (size_t)a.B * a.H * ((a.T + 31) / 32) < 1u << 24;
+  return a.B > 0 && a.B < 1 << 24 && a.T > 0 && a.Hk > 0 && a.H > 0 && a.H % a.Hk == 0 && a.hd > 0 && a.hd <= kAttnTrainHead &&
+         a.T <= 1 << 24 && a.qkv_cols <= 1 << 20 && a.out_cols <= 1 << 20 &&
+         (size_t)a.B * (a.H + a.Hk) * ((a.T + 31) / 32) < 1u << 24;
 }
 
 namespace {

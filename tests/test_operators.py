@@ -167,9 +167,9 @@ def test_attention_lengths(fhp, be, T, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("hd", [1, 5, 8, 20, 32, 36, 40, 72, 80, 100, 128])
+@pytest.mark.parametrize("hd", [1, 5, 8, 20, 32, 36, 40, 72, 80, 90, 100, 128])
 def test_attention_head_sizes(fhp, be, hd, dtype):
-    # 5, 20 (bf16) and 36 (bf16) are no multiple of 16 bytes
+    # 5, 90, 20 (bf16) and 36 (bf16) are no multiple of 16 bytes
     attention_case(fhp, be, 1, 75, 4, 2, hd, dtype, seed=hd)
 
 
