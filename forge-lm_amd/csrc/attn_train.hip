@@ -304,21 +304,24 @@ __global__ __launch_bounds__(256) void k_attn_split(const AttnTrain a, const Spl
 }
 
 // Whether `blocks` blocks of 128 rows are so few that KS 4 pays: a wave's chain of steps is a quarter as long,
-// and every tile is fetched for 32 rows instead of 128.  us with KS 1 and KS 4, 12 heads of 64 but where said:
-//   bf16  192 blocks (2 x 1024) 20 and 16, 256 (4 x 1024, 8 heads) 21 and 23, 384 (4 x 1024) 24 and 29
+// and every tile is fetched for 32 rows instead of 128.  Fewer in bf16 where T is short: its chains cost little
+// beside the join.  us with KS 1 and KS 4, 12 heads of 64 but where said:
+//   bf16  192 blocks (2 x 1024) 20 and 16, 256 (4 x 1024, 8 heads) 21 and 23, 384 (4 x 1024) 24 and 29; heads of 32:
+//         256 (2 x 1024, 16 heads) 17 and 14; shorter T: 96 (2 x 512) 11.1 and 9.9, 192 (4 x 512) 12.3 and 12.2, (8 x
+//         256) 8.3 and 10, (16 x 128) 6.6 and 8.7; heads of 128: 96 (2 x 700, 8 heads) 22 and 17, 192 (4 x 400) 16 and 23
 //   fp32  192 blocks 87 and 53, 384 100 and 89, 768 153 and 165; heads of 128: 256 blocks (2 x 2000, 8 heads) 291
 //         and 228, 384 (8 x 300, 16 heads) 73 and 98
 template <typename K, int HD>
-bool few_blocks(size_t blocks, int cus) {
-  const size_t quarters = std::is_same_v<K, AtF32> ? HD > 64 ? 5 : 8 : 4;  // of the CUs
-  return 4 * blocks < quarters * cus;
+bool few_blocks(size_t blocks, int T, int cus) {
+  if (std::is_same_v<K, AtF32>) return 4 * blocks < (HD > 64 ? 5 : 8) * (size_t)cus;
+  return 4 * 1024 * blocks < (HD > 32 ? 4 : 5) * (size_t)cus * (T < 1024 ? T : 1024);
 }
 
 template <typename K, int HD, bool VEC>
 void forward_hd(hipStream_t st, const AttnTrain& a, int cus) {
   const size_t g = (size_t)a.B * a.H, wide = (size_t)((a.T + 127) / 128) * g, narrow = (size_t)((a.T + 31) / 32) * g;
   if constexpr (VEC && K::kParts == 1) {  // (parts: where blocks are many, attn_train_split)
-    if (few_blocks<K, HD>(wide, cus)) {
+    if (few_blocks<K, HD>(wide, a.T, cus)) {
       hipLaunchKernelGGL((k_attn_forward<K, HD, 4, VEC>), dim3((unsigned)narrow), dim3(256), 0, st, a);
       return;
     }
