@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, K::kParts * HD * KS >= 512 && sizeof(typename 
     }
     const int i = lane & 31;
     const float sum = ol[i] + ol[32 + i] + ol[64 + i] + ol[96 + i];
-    if (__syncthreads_or(at_spoilt(o)) && w == 0) forward_again<O, HD>(a, b, h, t0, len, mx, sum, lane);
+    if (at_block_spoilt(at_spoilt(o)) && w == 0) forward_again<O, HD>(a, b, h, t0, len, mx, sum, lane);
   }
 }
 

@@ -483,6 +483,13 @@ __device__ __forceinline__ bool at_spoilt(const at_f32x16 (&acc)[N]) {
     for (int r = 0; r < 16; r++) s = fmaf(acc[dt][r], 0.f, s);
   return __builtin_amdgcn_ballot_w64(s != s) != 0;
 }
+// The same of any wave of a block whose waves have stored parts of the same rows; then those stores have arrived.
+__device__ __forceinline__ bool at_block_spoilt(bool spoilt) {
+  if (!__syncthreads_or(spoilt)) return false;
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  __syncthreads();
+  return true;
+}
 // Whether some dim of the lane's is not finite in a hidden row of x (n rows, stride apart) and finite in all
 // that its own row i sees: rows 0 .. i, or (UP) i .. n - 1.
 template <typename O, bool UP>

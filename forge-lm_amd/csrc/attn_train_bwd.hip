@@ -247,7 +247,7 @@ __device__ __forceinline__ void backward_q(const AttnTrain& a, int block, int bl
     if (at_spoilt(dq)) backward_q_again<O, HD>(a, b, h, qw0, len, lane);
   } else {
     join_store<O, HD>(reinterpret_cast<float*>(smem), dq, a.scale, dst, t0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
-    if (__syncthreads_or(at_spoilt(dq)) && w == 0) backward_q_again<O, HD>(a, b, h, t0, len, lane);
+    if (at_block_spoilt(at_spoilt(dq)) && w == 0) backward_q_again<O, HD>(a, b, h, t0, len, lane);
   }
 }
 
@@ -412,7 +412,7 @@ __device__ __forceinline__ void backward_kv(const AttnTrain& a, int block, int b
     float* os = reinterpret_cast<float*>(smem);
     join_store<O, HD>(os, dk, a.scale, dst, k0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
     join_store<O, HD>(os, dv, 1.f, dstv, k0, len, a.T, a.qkv_cols, a.hd, w, lane, tid);
-    if (__syncthreads_or(at_spoilt(dk) || at_spoilt(dv)) && w == 0) backward_kv_again<O, HD>(a, b, kvh, k0, len, lane);
+    if (at_block_spoilt(at_spoilt(dk) || at_spoilt(dv)) && w == 0) backward_kv_again<O, HD>(a, b, kvh, k0, len, lane);
   }
 }
 
