@@ -594,6 +594,42 @@ def test_a_training_step_with_both(fhp):
     ops.Dispose()
 
 
+@pytest.mark.gpu
+def test_two_contexts_at_once(fhp, be):
+    # each has its own stream, scratch and result: interleaved calls of two threads give what each gives alone
+    import threading
+
+    def work(b, seed, out):
+        r = np.random.default_rng(seed)
+        B, T, H, hd, V, K = 2, 300, 3, 64, 900, 4
+        x = fhp.DeviceBuffer.from_array(b, r.normal(0, 1, (B * T, 3 * H * hd)).astype(np.float32))
+        d = fhp.DeviceBuffer.from_array(b, r.normal(0, 1, (B * T, H * hd)).astype(np.float32))
+        z = fhp.DeviceBuffer.from_array(b, r.normal(0, 2, (T, V)).astype(np.float32))
+        ids = fhp.DeviceBuffer.from_array(b, r.integers(0, V, (T, K)).astype(np.int32))
+        top = fhp.DeviceBuffer.from_array(b, r.normal(0, 2, (T, K)).astype(np.float32))
+        o, l, g = fhp.DeviceBuffer(b, d.nbytes), fhp.DeviceBuffer(b, 4 * B * H * T), fhp.DeviceBuffer(b, x.nbytes)
+        targets = r.integers(0, V, T)
+        for _ in range(20):
+            b.attention_forward(x, o, l, B, T, H, hd)
+            loss = b.distill_loss(z, targets, ids, top, None, T, V, K, temperature=2.0, alpha=0.5)
+            b.attention_backward(d, x, o, l, g, B, T, H, hd)
+            out.append((loss, g.read(np.float32, x.nbytes // 4).tobytes()))
+        for buf in (x, d, z, ids, top, o, l, g):
+            buf.free()
+
+    with fhp.HipBackend(0) as other:
+        alone, together = [[], []], [[], []]
+        for b, seed, out in ((be, 1, alone[0]), (other, 2, alone[1])):
+            work(b, seed, out)
+        threads = [threading.Thread(target=work, args=(b, s, out)) for b, s, out in ((be, 1, together[0]), (other, 2, together[1]))]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+    for a, g in zip(alone, together):
+        assert len(g) == 20 and all(x == a[0] for x in a + g)
+
+
 # ---- refusals (before any device work) --------------------------------------------------------------------
 
 class Calls:
